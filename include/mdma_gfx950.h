@@ -362,6 +362,93 @@ int mdma_gfx950_set_replay_params(mdma_ctx *ctx, const mdma_buf *params, uint64_
  * Applies to one launch; not allowed during graph capture. */
 int mdma_gfx950_time_next_gemv(mdma_ctx *ctx, void *start_event, void *stop_event);
 
+/* ---- extras for a batch of requests ----
+ * A paged KV cache, attention over it and low-rank adapters, for callers that
+ * serve many requests at once (no counterparts in the reference, whose cache
+ * is one contiguous row of positions per sequence, src/kv_cache.rs:16-301).
+ * All state that changes from step to step (tables, lengths, ids) is in device
+ * memory, so a captured graph of these calls replays with what they hold then;
+ * sequence, page, layer and slot numbers count from 0, and 0xffffffff names
+ * none. Every activation mode runs the same arithmetic here. Buffers a call
+ * writes may not overlap its other buffers unless it says so.
+ *
+ * The cache: per layer n_pages pages of page_len positions (a power of two, 16
+ * to 256) of kv_width f16 (n_kv_heads * head_dim, a multiple of 8), k and v
+ * each [n_layers][n_pages][page_len][kv_width], 16-byte aligned. Sequence s
+ * (of n_seqs <= 1024) holds lens[s] positions, positions [i * page_len,
+ * (i + 1) * page_len) in page table[s][i] of its max_pages entries; one table
+ * serves all layers. refs[p] counts the table entries in use that name page
+ * p (0: free). An empty cache: table 0xffffffff, lens and refs 0. Entries that
+ * name no page of the pool are skipped wherever they are met: their positions
+ * are not read, written, counted or copied; a length past max_pages * page_len
+ * is read as that. */
+typedef struct {
+    mdma_buf *k, *v;
+    mdma_buf *table; /* u32 [n_seqs][max_pages] */
+    mdma_buf *lens;  /* u32 [n_seqs] */
+    mdma_buf *refs;  /* u32 [n_pages] */
+    uint64_t n_layers, n_pages, page_len, kv_width, n_seqs, max_pages;
+} mdma_kv_pages;
+
+/* Every sequence s becomes the first min(keep[s], lens[from[s]]) positions of
+ * sequence from[s], all read as they were before the call: from[s] = s with a
+ * smaller keep cuts a sequence, an id that names none frees it, the same id
+ * several times forks it, any order reorders a beam. from, keep: u32 [n_seqs]
+ * (keep NULL: whole sequences). Pages are shared, not copied; entries past a
+ * sequence's pages become 0xffffffff, and refs is counted anew. */
+int mdma_gfx950_kv_pages_fork(mdma_ctx *ctx, const mdma_kv_pages *pages, const mdma_buf *from, const mdma_buf *keep);
+/* Room for grow[s] more positions (u32 [n_seqs]) in every sequence: a partly
+ * filled last page that other sequences hold too is copied first, the positions held
+ * (all layers; of the holders that grow, the last goes on in place when no other is left),
+ * further pages are taken, and lens[s] grows. Pages are the lowest free ids, in
+ * sequence order. status[s] (u32 [n_seqs], written) is 0, 2 where the sequence
+ * would pass max_pages (it stays as it is), or 1 from the first sequence on
+ * for which free pages run out (it and all after it that asked stay as they are). */
+int mdma_gfx950_kv_pages_grow(mdma_ctx *ctx, const mdma_kv_pages *pages, const mdma_buf *grow, mdma_buf *status);
+/* The L pages in use move to the ids 0 .. L - 1: those at L and past it,
+ * ascending, into the free ids below, ascending (contents of all layers, table
+ * entries and refs). n_live (u32, written; NULL: not wanted) is L. Prefix
+ * lists a caller keeps apart from the table are not renumbered. */
+int mdma_gfx950_kv_pages_compact(mdma_ctx *ctx, const mdma_kv_pages *pages, mdma_buf *n_live);
+/* rope_kv_write for the batch: q [n_seqs][n_new][heads * head_dim], k and v
+ * [n_seqs][n_new][kv_width] f32 (n_new from k's length); new token j of
+ * sequence s is position lens[s] - n_new + j (its room made by kv_pages_grow
+ * before), q rotated in place, the rotated k and v stored in layer's pages
+ * (rounded to f16; k itself is not changed). The angles are rope's: the f32
+ * product of the position and the f32 frequency. A token before position 0
+ * (an empty slot of a padded batch) is left alone. */
+int mdma_gfx950_rope_kv_write_paged(mdma_ctx *ctx, mdma_buf *q, const mdma_buf *k, const mdma_buf *v,
+                                    const mdma_kv_pages *pages, uint64_t layer, const mdma_rope_spec *spec);
+/* Causal attention of the batch's last n_new tokens (n_new from q's length):
+ * q, o [n_seqs][n_new][n_q_heads * head_dim] f32; token j of sequence s
+ * attends to positions 0 .. lens[s] - n_new + j of its pages, scale
+ * 1/sqrt(head_dim); one that sees no position gets zeros. head_dim a
+ * multiple of 8, at most 256. prefix (u32 page ids; NULL: none): the first
+ * prefix->len / 4 pages of every sequence, in place of those table entries,
+ * their keys and values read once for the whole batch (a view of a table row
+ * is one way to pass a shared prompt's pages). Sequences shorter than the prefix
+ * see the positions they hold. */
+int mdma_gfx950_attn_paged(mdma_ctx *ctx, const mdma_buf *q, const mdma_kv_pages *pages, uint64_t layer,
+                           const mdma_buf *prefix, const mdma_attn_spec *spec, mdma_buf *o);
+
+/* Low-rank adapters for one projection [n_out, n_in]: n_slots slots of up to
+ * max_rank (at most 256), F32 or F16 (dtype) values, in device memory of
+ * the set's own (charged to the budget), empty at first. */
+typedef struct mdma_lora mdma_lora;
+int mdma_gfx950_lora_new(mdma_ctx *ctx, int32_t dtype, uint64_t n_in, uint64_t n_out, uint64_t max_rank,
+                         uint64_t n_slots, mdma_lora **out);
+/* Host values a [rank, n_in] and b [n_out, rank] into a slot (rank 0 empties
+ * it), after the work queued so far. */
+int mdma_gfx950_lora_load(mdma_lora *lora, uint64_t slot, const void *a, const void *b, uint64_t rank, float scale);
+/* y[t] = base[t] + scale * b (a x[t]) with the adapter of slot ids[t] (u32
+ * [T]); y[t] = base[t] where ids[t] names no slot, or an empty one. x [T,
+ * n_in], base and y [T, n_out] f32, T from x's length; y may be base
+ * itself. Sums are f32 in an order fixed by the call's sizes and ids. */
+int mdma_gfx950_lora_add(mdma_ctx *ctx, const mdma_lora *lora, const mdma_buf *ids, const mdma_buf *x,
+                         const mdma_buf *base, mdma_buf *y);
+/* Graphs that use the set must not be launched afterwards. */
+int mdma_gfx950_lora_free(mdma_lora *lora);
+
 /* ---- Llama decoding: the hot path's caller ----
  * Model / KvCache / Workspace / inference::generate (src/model.rs:41-468,
  * src/kv_cache.rs:16-301, src/inference.rs:44-124). A session owns the f16 KV

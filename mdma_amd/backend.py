@@ -68,6 +68,11 @@ class KvViewC(C.Structure):
     _fields_ = [("k", _P), ("v", _P), ("len", _U64)]
 
 
+class KvPagesC(C.Structure):
+    _fields_ = [(n, _P) for n in ("k", "v", "table", "lens", "refs")] + \
+        [(n, _U64) for n in ("n_layers", "n_pages", "page_len", "kv_width", "n_seqs", "max_pages")]
+
+
 _SIGS = {
     "create": [C.c_int, _P], "destroy": [_P], "last_error": [],
     "device_label": [_P, C.c_char_p, C.c_size_t], "total_device_bytes": [_P],
@@ -94,6 +99,10 @@ _SIGS = {
     "prepared_bytes": [_I32, _U64, _U64],
     "pack_weight": [_I32, _U64, _U64, _P, _U64, _P, _U64],
     "unpack_weight": [_I32, _U64, _U64, _P, _U64, _P, _U64],
+    "kv_pages_fork": [_P, _P, _P, _P], "kv_pages_grow": [_P, _P, _P, _P], "kv_pages_compact": [_P, _P, _P],
+    "rope_kv_write_paged": [_P, _P, _P, _P, _P, _U64, _P], "attn_paged": [_P, _P, _P, _U64, _P, _P, _P],
+    "lora_new": [_P, _I32, _U64, _U64, _U64, _U64, _P], "lora_load": [_P, _U64, _P, _P, _U64, _F],
+    "lora_add": [_P, _P, _P, _P, _P, _P], "lora_free": [_P],
 }
 _RESTYPES = {"prepared_bytes": _U64, "destroy": None, "graph_destroy": None, "last_error": C.c_char_p, "total_device_bytes": _U64, "max_head_dim": _U64,
              "kv_elem_bytes": _U64, "stream": _P, "buf_len": _U64, "supports_weight_dtype": C.c_int}
@@ -204,6 +213,72 @@ class KvView:
     k: Buf
     v: Buf
     len: int
+
+
+NO_PAGE = 0xffffffff  # a table entry that names no page, an id that names no sequence or adapter slot
+
+
+@dataclass
+class KvPages:
+    """A paged KV cache (mdma_kv_pages): the pools k and v, f16 [n_layers]
+    [n_pages][page_len][kv_width], and the books, uint32: table [n_seqs]
+    [max_pages], lens [n_seqs], refs [n_pages]. `Gfx950Backend.kv_pages`
+    allocates an empty one."""
+    k: Buf
+    v: Buf
+    table: Buf
+    lens: Buf
+    refs: Buf
+    n_layers: int
+    n_pages: int
+    page_len: int
+    kv_width: int
+    n_seqs: int
+    max_pages: int
+
+    def c(self) -> KvPagesC:
+        return KvPagesC(*(b.handle for b in (self.k, self.v, self.table, self.lens, self.refs)), self.n_layers,
+                        self.n_pages, self.page_len, self.kv_width, self.n_seqs, self.max_pages)
+
+
+class Lora:
+    """The low-rank adapters of one projection (mdma_lora); freed on
+    close()/GC. See Gfx950Backend.lora."""
+
+    def __init__(self, backend: "Gfx950Backend", dtype: int, n_in: int, n_out: int, max_rank: int, n_slots: int):
+        self.handle = None
+        self.backend = backend
+        if dtype not in (GGML_F32, GGML_F16):
+            raise _ERR_TYPES[3](3, f"lora_new: dtype {dtype}")
+        self.np_dtype = np.float16 if dtype == GGML_F16 else np.float32
+        self.n_in, self.n_out = n_in, n_out
+        h = C.c_void_p()
+        _check(lib().mdma_gfx950_lora_new(backend.ctx, dtype, n_in, n_out, max_rank, n_slots, C.byref(h)))
+        self.handle = h.value
+
+    def load(self, slot: int, a, b, scale: float = 1.0):
+        """a [rank, n_in] and b [n_out, rank] of the set's dtype into a slot;
+        None for both empties it."""
+        if a is None and b is None:
+            _check(lib().mdma_gfx950_lora_load(self.handle, slot, None, None, 0, scale))
+            return
+        a, b = np.ascontiguousarray(a, self.np_dtype), np.ascontiguousarray(b, self.np_dtype)
+        if a.ndim != 2 or a.shape[1] != self.n_in or b.shape != (self.n_out, a.shape[0]):
+            raise _ERR_TYPES[2](2, f"lora_load: a {a.shape} and b {b.shape} are not [rank, {self.n_in}] and "
+                                   f"[{self.n_out}, rank]")
+        _check(lib().mdma_gfx950_lora_load(self.handle, slot, a.ctypes.data, b.ctypes.data, a.shape[0], scale))
+
+    def close(self):
+        if self.handle:
+            h, self.handle = self.handle, None
+            if self.backend.ctx is not None:
+                _check(lib().mdma_gfx950_lora_free(h))
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class Gfx950Backend:
@@ -406,6 +481,53 @@ class Gfx950Backend:
         view = KvViewC(kv.k.handle, kv.v.handle, kv.len)
         s = AttnSpecC(spec.head_dim, spec.n_q_heads, spec.n_kv_heads)
         _check(lib().mdma_gfx950_attn(self.ctx, q.handle, C.byref(view), C.byref(s), o.handle))
+
+    # -- a batch of requests: paged cache and adapters --
+    def kv_pages(self, n_layers: int, n_pages: int, page_len: int, kv_width: int, n_seqs: int,
+                 max_pages: int) -> KvPages:
+        """An empty paged cache (uploads its books: not during a capture)."""
+        pool = n_layers * n_pages * page_len * kv_width * 2
+        p = KvPages(self.alloc(pool, POOL_KV), self.alloc(pool, POOL_KV), self.alloc(n_seqs * max_pages * 4, POOL_KV),
+                    self.alloc(n_seqs * 4, POOL_KV), self.alloc(n_pages * 4, POOL_KV), n_layers, n_pages, page_len,
+                    kv_width, n_seqs, max_pages)
+        self.upload(p.table, 0, np.full(n_seqs * max_pages, NO_PAGE, np.uint32))
+        self.upload(p.lens, 0, np.zeros(n_seqs, np.uint32))
+        self.upload(p.refs, 0, np.zeros(n_pages, np.uint32))
+        return p
+
+    def kv_pages_fork(self, pages: KvPages, from_: Buf, keep: "Buf | None" = None):
+        """Sequence s becomes the first keep[s] positions of sequence from_[s] (uint32 [n_seqs] each): forks,
+        cuts, reorders and frees sequences without copying a page."""
+        _check(lib().mdma_gfx950_kv_pages_fork(self.ctx, C.byref(pages.c()), from_.handle,
+                                               keep.handle if keep is not None else None))
+
+    def kv_pages_grow(self, pages: KvPages, grow: Buf, status: Buf):
+        """Room for grow[s] more positions in every sequence; status[s]: 0, 1 (no free pages) or 2 (max_pages)."""
+        _check(lib().mdma_gfx950_kv_pages_grow(self.ctx, C.byref(pages.c()), grow.handle, status.handle))
+
+    def kv_pages_compact(self, pages: KvPages, n_live: "Buf | None" = None):
+        """The pages in use move to the lowest ids; their number into n_live (one uint32)."""
+        _check(lib().mdma_gfx950_kv_pages_compact(self.ctx, C.byref(pages.c()),
+                                                  n_live.handle if n_live is not None else None))
+
+    def rope_kv_write_paged(self, q: Buf, k: Buf, v: Buf, pages: KvPages, layer: int, spec: RopeSpec):
+        s = RopeSpecC(spec.head_dim, spec.theta)
+        _check(lib().mdma_gfx950_rope_kv_write_paged(self.ctx, q.handle, k.handle, v.handle, C.byref(pages.c()),
+                                                     layer, C.byref(s)))
+
+    def attn_paged(self, q: Buf, pages: KvPages, layer: int, prefix: "Buf | None", spec: AttnSpec, o: Buf):
+        """Causal attention of the batch's last tokens; prefix: page ids shared by every sequence, read once."""
+        s = AttnSpecC(spec.head_dim, spec.n_q_heads, spec.n_kv_heads)
+        _check(lib().mdma_gfx950_attn_paged(self.ctx, q.handle, C.byref(pages.c()), layer,
+                                            prefix.handle if prefix is not None else None, C.byref(s), o.handle))
+
+    def lora(self, dtype: int, n_in: int, n_out: int, max_rank: int, n_slots: int) -> Lora:
+        """Low-rank adapters for one projection: n_slots empty slots of up to max_rank (GGML_F32 or GGML_F16)."""
+        return Lora(self, dtype, n_in, n_out, max_rank, n_slots)
+
+    def lora_add(self, lora: Lora, ids: Buf, x: Buf, base: Buf, y: Buf):
+        """y = base + scale * b (a x) with the adapter of slot ids[t] (uint32 [T]) for every token t; y may be base."""
+        _check(lib().mdma_gfx950_lora_add(self.ctx, lora.handle, ids.handle, x.handle, base.handle, y.handle))
 
     # -- extras --
     def greedy(self, logits: Buf, offset: int = 0, n: int | None = None) -> int:

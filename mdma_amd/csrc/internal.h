@@ -503,4 +503,42 @@ void launch_step_record(mdma_ctx *ctx, uint32_t *params, const uint32_t *cur, co
 void launch_argmax_rows(mdma_ctx *ctx, const float *x, uint64_t rows, uint64_t n, uint32_t *idx,
                         uint32_t *flag);
 
+// ---- a batch of requests: paged cache and adapters (serve.cpp) ----
+struct PagedView;
+// A paged cache's books and pools, all layers (checked by the caller: n_seqs
+// <= 1024, width a multiple of 8, page offsets in 64 bits).
+struct KvBooks {
+  uint16_t *k, *v;
+  uint32_t *table, *lens, *refs;
+  uint32_t n_layers, n_pages, page_shift, width, n_seqs, max_pages;
+};
+constexpr uint64_t KV_MAX_SEQS = 1024;  // a thread each in grow's workgroup
+// kv_pages.hip; tmp: that many bytes of device space.
+uint64_t kv_fork_scratch(uint64_t n_seqs, uint64_t max_pages);
+void launch_kv_fork(mdma_ctx *ctx, const KvBooks &b, const uint32_t *from, const uint32_t *keep, uint32_t *tmp);
+uint64_t kv_grow_scratch(uint64_t n_seqs, uint64_t n_pages);
+void launch_kv_grow(mdma_ctx *ctx, const KvBooks &b, const uint32_t *grow, uint32_t *tmp, uint32_t *status);
+uint64_t kv_compact_scratch(uint64_t n_pages);
+void launch_kv_compact(mdma_ctx *ctx, const KvBooks &b, uint32_t *tmp, uint32_t *n_live);
+void launch_rope_kv_paged(mdma_ctx *ctx, float *q, const float *k, const float *v, const PagedView &kv, uint32_t n_new,
+                          uint32_t q_heads, uint32_t kv_heads, uint32_t hd, const float *tab);
+// attn_paged.hip.
+void launch_attn_paged(mdma_ctx *ctx, const float *q, const PagedView &kv, uint32_t n_new, uint32_t q_heads,
+                       uint32_t kv_heads, uint32_t hd, float *o);
+// lora.hip. A slot's A is [rank_pad][in_pad], its B [n_out][stride] (stride:
+// its rank in whole 16s), both padded with zeros; rank 0: no adapter.
+struct LoraSlot {
+  uint32_t rank, stride;
+  float scale;
+};
+struct LoraView {
+  int32_t dtype;
+  uint32_t n_in, n_out, in_pad, rank_pad, n_slots;
+  const void *a, *b;
+  const LoraSlot *info;
+};
+uint64_t lora_scratch(const LoraView &w, uint64_t T);
+void launch_lora(mdma_ctx *ctx, const LoraView &w, const uint32_t *ids, uint32_t T, const float *x, const float *base,
+                 float *y, float *u);
+
 }  // namespace mdma

@@ -3,6 +3,8 @@
 #pragma once
 #include <hip/hip_ext.h>
 
+#include <algorithm>
+
 #include "internal.h"
 
 namespace mdma {

@@ -1,0 +1,320 @@
+// Page tables of a paged KV cache on the device: sequences copied, cut and
+// freed by their table rows (fork), lengthened (grow), live pages moved to the
+// lowest ids (compact); and the rotated K / V rows of new tokens stored into
+// their pages.
+//
+// The tables are a few KB to a few MB, so the calls are bound by launches and
+// by the latency of one workgroup's scans; the copies they cause (a shared
+// last page, a page moved) run on the whole chip, in 16-byte pieces.
+#include "kernels.h"
+#include "paged.h"
+
+namespace mdma {
+namespace {
+
+constexpr uint32_t BOOK_WG = 1024;  // threads of a bookkeeping workgroup
+
+// Exclusive prefix sum of v over the workgroup; *total = the sum.
+__device__ __forceinline__ uint32_t scan_wg(uint32_t v, uint32_t *total) {
+  __shared__ uint32_t wsum[BOOK_WG / 64];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t y = __shfl_up(x, d, 64);
+    if (lane >= (uint32_t)d) x += y;
+  }
+  __syncthreads();  // (the last call's reads of wsum)
+  if (lane == 63) wsum[wave] = x;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < BOOK_WG / 64; w++) {
+    const uint32_t s = wsum[w];
+    if (w < wave) before += s;
+    all += s;
+  }
+  *total = all;
+  return before + x - v;
+}
+
+// fork, first half: every new row into tmp, from the old rows; refs cleared.
+__global__ __launch_bounds__(256) void fork_gather_kernel(const uint32_t *__restrict__ table,
+                                                          const uint32_t *__restrict__ lens,
+                                                          const uint32_t *__restrict__ from,
+                                                          const uint32_t *__restrict__ keep, uint32_t n_seqs,
+                                                          uint32_t max_pages, uint32_t page_shift, uint32_t n_pages,
+                                                          uint32_t *__restrict__ tmp_table,
+                                                          uint32_t *__restrict__ tmp_lens, uint32_t *__restrict__ refs) {
+  const uint64_t step = (uint64_t)gridDim.x * blockDim.x, at = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  for (uint64_t i = at; i < n_pages; i += step) refs[i] = 0;
+  const uint64_t cap = (uint64_t)max_pages << page_shift;
+  for (uint64_t e = at; e < (uint64_t)n_seqs * max_pages; e += step) {
+    const uint32_t s = e / max_pages, i = e % max_pages, f = from[s];
+    uint32_t n = 0;
+    if (f < n_seqs) {
+      n = (uint32_t)min((uint64_t)lens[f], cap);
+      if (keep) n = min(n, keep[s]);
+    }
+    const bool held = ((uint64_t)i << page_shift) < n;
+    tmp_table[e] = held ? table[(uint64_t)f * max_pages + i] : NO_PAGE;
+    if (i == 0) tmp_lens[s] = n;
+  }
+}
+// fork, second half: the rows back, their pages counted.
+__global__ __launch_bounds__(256) void fork_store_kernel(const uint32_t *__restrict__ tmp_table,
+                                                         const uint32_t *__restrict__ tmp_lens, uint32_t n_seqs,
+                                                         uint32_t max_pages, uint32_t n_pages,
+                                                         uint32_t *__restrict__ table, uint32_t *__restrict__ lens,
+                                                         uint32_t *__restrict__ refs) {
+  const uint64_t step = (uint64_t)gridDim.x * blockDim.x;
+  for (uint64_t e = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; e < (uint64_t)n_seqs * max_pages; e += step) {
+    const uint32_t id = tmp_table[e];
+    table[e] = id;
+    if (id < n_pages) atomicAdd(refs + id, 1u);  // (whole numbers: any order gives the same count)
+    if (e < n_seqs) lens[e] = tmp_lens[e];
+  }
+}
+
+// grow, one workgroup, a sequence a thread. copies[s] = {source page,
+// destination page, positions} for a shared last page (positions 0: none).
+__global__ __launch_bounds__(BOOK_WG) void grow_kernel(uint32_t *__restrict__ table, uint32_t *__restrict__ lens,
+                                                       uint32_t *__restrict__ refs, const uint32_t *__restrict__ grow,
+                                                       uint32_t n_seqs, uint32_t max_pages, uint32_t page_shift,
+                                                       uint32_t n_pages, uint32_t *__restrict__ free_ids,
+                                                       uint32_t *__restrict__ copies, uint32_t *__restrict__ status) {
+  __shared__ uint32_t shared_last[BOOK_WG];
+  const uint32_t s = threadIdx.x, page_mask = (1u << page_shift) - 1;
+  uint32_t len = 0, g = 0, before = 0, extra = 0, last = NO_PAGE;
+  bool grows = false, over = false;
+  if (s < n_seqs) {
+    len = lens[s];
+    g = grow[s];
+    const uint64_t end = (uint64_t)len + g;
+    over = g && end > ((uint64_t)max_pages << page_shift);
+    grows = g && !over;
+    if (grows) {
+      before = (uint32_t)(((uint64_t)len + page_mask) >> page_shift);
+      extra = (uint32_t)((end + page_mask) >> page_shift) - before;
+      if (len & page_mask) last = table[(uint64_t)s * max_pages + before - 1];
+      if (last >= n_pages) last = NO_PAGE;
+    }
+  }
+  // The holders of a partly filled page copy it in sequence order, all but
+  // the last one to hold it, which goes on in place.
+  shared_last[s] = last;
+  __syncthreads();
+  bool cow = false;
+  if (last != NO_PAGE) {
+    const uint32_t held = refs[last];
+    if (held > 1) {
+      uint32_t earlier = 0;
+      for (uint32_t i = 0; i < s; i++) earlier += shared_last[i] == last;
+      cow = earlier + 1 < held;
+    }
+  }
+  const uint32_t need = grows ? extra + cow : 0;
+  uint32_t total;
+  const uint32_t start = scan_wg(need, &total);
+  // The lowest free ids, as many as are needed.
+  uint32_t found = 0;
+  for (uint32_t p0 = 0; p0 < n_pages && found < total; p0 += BOOK_WG) {  // (uniform)
+    const uint32_t p = p0 + s;
+    const bool is_free = p < n_pages && refs[p] == 0;
+    uint32_t n;
+    const uint32_t at = found + scan_wg(is_free, &n);
+    if (is_free && at < total) free_ids[at] = p;
+    found += n;
+  }
+  __threadfence_block();
+  __syncthreads();  // free_ids written, refs read
+  // In order, until one does not fit: it and all that grow after it stay as they are.
+  const bool fits = grows && (uint64_t)start + need <= found;
+  if (s < n_seqs) {
+    uint32_t *row = table + (uint64_t)s * max_pages;
+    uint32_t rows = 0, dst = NO_PAGE;
+    if (fits) {
+      if (cow) {
+        dst = free_ids[start];
+        rows = len & page_mask;
+        row[before - 1] = dst;
+        refs[dst] = 1;
+        atomicSub(refs + last, 1u);
+      }
+      for (uint32_t e = 0; e < extra; e++) {
+        const uint32_t id = free_ids[start + cow + e];
+        row[before + e] = id;
+        refs[id] = 1;
+      }
+      lens[s] = len + g;
+    }
+    copies[3 * s] = last;
+    copies[3 * s + 1] = dst;
+    copies[3 * s + 2] = rows;
+    status[s] = fits || !g ? 0 : over ? 2 : 1;
+  }
+}
+
+// The rows copies[] names, in every layer of both pools: a workgroup per
+// (sequence, layer, pool). Sources and destinations are different pages.
+__global__ __launch_bounds__(256) void grow_copy_kernel(uint16_t *__restrict__ k, uint16_t *__restrict__ v,
+                                                        const uint32_t *__restrict__ copies, uint32_t n_pages,
+                                                        uint32_t page_shift, uint32_t width) {
+  const uint32_t s = blockIdx.x, rows = copies[3 * s + 2];
+  if (!rows) return;
+  uint16_t *pool = blockIdx.z ? v : k;
+  const uint64_t layer = (uint64_t)blockIdx.y * n_pages;
+  const uint4 *src = reinterpret_cast<const uint4 *>(pool + ((layer + copies[3 * s]) << page_shift) * width);
+  uint4 *dst = reinterpret_cast<uint4 *>(pool + ((layer + copies[3 * s + 1]) << page_shift) * width);
+  for (uint32_t i = threadIdx.x; i < rows * (width / 8); i += 256) dst[i] = src[i];
+}
+
+// compact, one workgroup: the live pages' count; pairs[i] = {live id at or
+// past it, free id below it}; remap of the ids from there on; refs moved.
+// head = {live pages, pairs}.
+__global__ __launch_bounds__(BOOK_WG) void compact_plan_kernel(uint32_t *__restrict__ refs, uint32_t n_pages,
+                                                               uint32_t *__restrict__ src, uint32_t *__restrict__ dst,
+                                                               uint32_t *__restrict__ remap, uint32_t *__restrict__ head,
+                                                               uint32_t *__restrict__ n_live) {
+  uint32_t mine = 0, live, n;
+  for (uint32_t p = threadIdx.x; p < n_pages; p += BOOK_WG) mine += refs[p] != 0;
+  scan_wg(mine, &live);
+  uint32_t n_src = 0, n_dst = 0;
+  for (uint32_t p0 = 0; p0 < n_pages; p0 += BOOK_WG) {  // (uniform)
+    const uint32_t p = p0 + threadIdx.x;
+    const bool in = p < n_pages, held = in && refs[p] != 0;
+    if (p0 < live) {
+      const bool hole = in && p < live && !held;
+      const uint32_t at = n_dst + scan_wg(hole, &n);
+      if (hole) dst[at] = p;
+      n_dst += n;
+    }
+    if (p0 + BOOK_WG > live) {
+      const bool moves = held && p >= live;
+      const uint32_t at = n_src + scan_wg(moves, &n);
+      if (moves) src[at] = p;
+      if (in && p >= live && !held) remap[p] = p;
+      n_src += n;
+    }
+  }
+  __threadfence_block();
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < n_src; i += BOOK_WG) {  // (n_src == n_dst)
+    const uint32_t a = src[i], b = dst[i];
+    remap[a] = b;
+    refs[b] = refs[a];
+    refs[a] = 0;
+  }
+  if (threadIdx.x == 0) {
+    head[0] = live;
+    head[1] = n_src;
+    if (n_live) *n_live = live;
+  }
+}
+// compact: table entries renumbered; pages copied, a (pair, layer, pool) at a
+// time per workgroup. Every source id is at or past the live count and every
+// destination below it, so the copies are independent.
+__global__ __launch_bounds__(256) void compact_move_kernel(uint16_t *__restrict__ k, uint16_t *__restrict__ v,
+                                                           uint32_t *__restrict__ table, uint64_t entries,
+                                                           const uint32_t *__restrict__ src,
+                                                           const uint32_t *__restrict__ dst,
+                                                           const uint32_t *__restrict__ remap,
+                                                           const uint32_t *__restrict__ head, uint32_t n_layers,
+                                                           uint32_t n_pages, uint32_t page_shift, uint32_t width) {
+  const uint32_t live = head[0], pairs = head[1];
+  for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < entries; e += (uint64_t)gridDim.x * 256) {
+    const uint32_t id = table[e];
+    if (id >= live && id < n_pages) table[e] = remap[id];
+  }
+  const uint64_t jobs = (uint64_t)pairs * n_layers * 2, page = (uint64_t)width << page_shift;
+  for (uint64_t j = blockIdx.x; j < jobs; j += gridDim.x) {
+    const uint32_t i = j / (2 * n_layers), r = j % (2 * n_layers);
+    uint16_t *pool = (r & 1 ? v : k) + (uint64_t)(r >> 1) * n_pages * page;
+    const uint4 *a = reinterpret_cast<const uint4 *>(pool + src[i] * page);
+    uint4 *b = reinterpret_cast<uint4 *>(pool + dst[i] * page);
+    for (uint32_t x = threadIdx.x; x < page / 8; x += 256) b[x] = a[x];
+  }
+}
+
+// rope_kv_kernel over a batch of sequences of their own lengths: new token j
+// of sequence s sits at position len - n_new + j. Positions below 0 (a
+// sequence shorter than n_new, an empty slot) are left alone.
+__global__ __launch_bounds__(256) void rope_kv_paged_kernel(float *__restrict__ q, const float *__restrict__ k,
+                                                            const float *__restrict__ v, PagedView kv, uint32_t n_new,
+                                                            uint32_t q_heads, uint32_t kv_heads, uint32_t hd,
+                                                            const float *__restrict__ tab) {
+  const uint32_t t = blockIdx.x, s = t / n_new, j = t % n_new, half = hd / 2;
+  const uint32_t len = kv.length(s);
+  if (len + j < n_new) return;
+  const uint32_t pos = len - n_new + j;
+  const float2 *cs = reinterpret_cast<const float2 *>(tab) + (uint64_t)pos * half;
+  const uint32_t id = kv.page(s, pos >> kv.page_shift);
+  const uint64_t row = kv.row(id, pos);
+  const uint32_t nq = q_heads * half, nk = kv_heads * half;
+  float2 *qr = reinterpret_cast<float2 *>(q) + (uint64_t)t * nq;
+  const float2 *kr = reinterpret_cast<const float2 *>(k) + (uint64_t)t * nk;
+  const float2 *vr = reinterpret_cast<const float2 *>(v) + (uint64_t)t * nk;
+  for (uint32_t p = blockIdx.y * 256 + threadIdx.x; p < nq + nk; p += gridDim.y * 256) {
+    if (p < nq) {
+      float2 x = qr[p];
+      const float2 c = cs[p % half];
+      rot(x.x, x.y, c.x, c.y);
+      qr[p] = x;
+    } else if (id != NO_PAGE) {
+      const uint32_t i = p - nq;
+      float2 x = kr[i];
+      const float2 c = cs[i % half], y = vr[i];
+      rot(x.x, x.y, c.x, c.y);
+      _Float16 *dk = reinterpret_cast<_Float16 *>(kv.k) + row + 2 * i, *dv = reinterpret_cast<_Float16 *>(kv.v) + row + 2 * i;
+      dk[0] = (_Float16)x.x;
+      dk[1] = (_Float16)x.y;
+      dv[0] = (_Float16)y.x;
+      dv[1] = (_Float16)y.y;
+    }
+  }
+}
+
+}  // namespace
+
+uint64_t kv_fork_scratch(uint64_t n_seqs, uint64_t max_pages) { return (n_seqs * max_pages + n_seqs) * 4; }
+void launch_kv_fork(mdma_ctx *ctx, const KvBooks &b, const uint32_t *from, const uint32_t *keep, uint32_t *tmp) {
+  const uint64_t entries = (uint64_t)b.n_seqs * b.max_pages, most = entries > b.n_pages ? entries : b.n_pages;
+  const uint32_t grid = (uint32_t)std::min<uint64_t>((most + 255) / 256, 1024);
+  uint32_t *tmp_lens = tmp + entries;
+  fork_gather_kernel<<<grid, 256, 0, ctx->stream>>>(b.table, b.lens, from, keep, b.n_seqs, b.max_pages, b.page_shift,
+                                                    b.n_pages, tmp, tmp_lens, b.refs);
+  fork_store_kernel<<<grid, 256, 0, ctx->stream>>>(tmp, tmp_lens, b.n_seqs, b.max_pages, b.n_pages, b.table, b.lens,
+                                                   b.refs);
+  hip_check(hipGetLastError(), "kv_pages_fork launch");
+}
+
+uint64_t kv_grow_scratch(uint64_t n_seqs, uint64_t n_pages) { return (n_pages + 3 * n_seqs) * 4; }
+void launch_kv_grow(mdma_ctx *ctx, const KvBooks &b, const uint32_t *grow, uint32_t *tmp, uint32_t *status) {
+  uint32_t *copies = tmp + b.n_pages;
+  grow_kernel<<<1, BOOK_WG, 0, ctx->stream>>>(b.table, b.lens, b.refs, grow, b.n_seqs, b.max_pages, b.page_shift,
+                                              b.n_pages, tmp, copies, status);
+  grow_copy_kernel<<<dim3(b.n_seqs, b.n_layers, 2), 256, 0, ctx->stream>>>(b.k, b.v, copies, b.n_pages, b.page_shift,
+                                                                           b.width);
+  hip_check(hipGetLastError(), "kv_pages_grow launch");
+}
+
+uint64_t kv_compact_scratch(uint64_t n_pages) { return (3 * n_pages + 2) * 4; }
+void launch_kv_compact(mdma_ctx *ctx, const KvBooks &b, uint32_t *tmp, uint32_t *n_live) {
+  uint32_t *src = tmp + 2, *dst = src + b.n_pages, *remap = dst + b.n_pages;
+  compact_plan_kernel<<<1, BOOK_WG, 0, ctx->stream>>>(b.refs, b.n_pages, src, dst, remap, tmp, n_live);
+  const uint64_t entries = (uint64_t)b.n_seqs * b.max_pages;
+  const uint64_t jobs = std::max<uint64_t>((uint64_t)(b.n_pages + 1) / 2 * b.n_layers * 2, (entries + 255) / 256);
+  compact_move_kernel<<<(uint32_t)std::min<uint64_t>(jobs, (uint64_t)ctx->cu_count * 8), 256, 0, ctx->stream>>>(
+      b.k, b.v, b.table, entries, src, dst, remap, tmp, b.n_layers, b.n_pages, b.page_shift, b.width);
+  hip_check(hipGetLastError(), "kv_pages_compact launch");
+}
+
+void launch_rope_kv_paged(mdma_ctx *ctx, float *q, const float *k, const float *v, const PagedView &kv, uint32_t n_new,
+                          uint32_t q_heads, uint32_t kv_heads, uint32_t hd, const float *tab) {
+  const uint32_t pairs = (q_heads + kv_heads) * (hd / 2);
+  rope_kv_paged_kernel<<<dim3(kv.n_seqs * n_new, (pairs + 1023) / 1024), 256, 0, ctx->stream>>>(q, k, v, kv, n_new,
+                                                                                               q_heads, kv_heads, hd, tab);
+  hip_check(hipGetLastError(), "rope_kv_write_paged launch");
+}
+
+}  // namespace mdma

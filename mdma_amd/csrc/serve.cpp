@@ -1,0 +1,370 @@
+// C-ABI entry points for a batch of requests: the paged KV cache and its
+// attention, and low-rank adapters. Shapes, sizes and overlaps are checked
+// here, so a malformed call never reaches a kernel; what device memory holds
+// (page ids, lengths, adapter ids) is checked by the kernels.
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+#include <memory>
+#include <new>
+#include <vector>
+
+#include "internal.h"
+#include "paged.h"
+
+using namespace mdma;
+
+struct mdma_lora {
+  mdma_ctx *ctx = nullptr;
+  LoraView view{};
+  uint64_t max_rank = 0;
+  mdma_buf *a = nullptr, *b = nullptr, *info = nullptr;
+  ~mdma_lora() {
+    for (mdma_buf *x : {a, b, info}) mdma_gfx950_free(x);
+  }
+};
+
+namespace {
+
+template <class F>
+int guarded(F &&f) {
+  try {
+    f();
+    return MDMA_OK;
+  } catch (const Error &e) {
+    set_last_error(e.msg);
+    return e.code;
+  } catch (const std::bad_alloc &) {
+    set_last_error("host allocation failed");
+    return MDMA_ERR_OUT_OF_MEMORY;
+  } catch (...) {
+    set_last_error("unknown failure");
+    return MDMA_ERR_BACKEND;
+  }
+}
+
+std::string fmt(const char *f, ...) __attribute__((format(printf, 1, 2)));
+std::string fmt(const char *f, ...) {
+  char b[512];
+  va_list ap;
+  va_start(ap, f);
+  vsnprintf(b, sizeof b, f, ap);
+  va_end(ap);
+  return b;
+}
+
+// The context's device current for the call, the caller's own afterwards.
+struct OnDevice {
+  int before = -1;
+  explicit OnDevice(mdma_ctx *ctx) {
+    hip_check(hipGetDevice(&before), "device");
+    if (before == ctx->device) before = -1;
+    else hip_check(hipSetDevice(ctx->device), "device");
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+uint64_t times(uint64_t a, uint64_t b, const char *op) {
+  if (a && b > UINT64_MAX / a) fail(MDMA_ERR_SIZE_OVERFLOW, fmt("%s: size overflows", op));
+  return a * b;
+}
+
+// A buffer of this context with at least `bytes` bytes, aligned to `align`.
+void check_buf(mdma_ctx *ctx, const char *op, const char *what, const mdma_buf *b, uint64_t bytes, uint64_t align) {
+  if (!b) shape_fail(fmt("%s: null %s", op, what));
+  if (b->ctx != ctx) shape_fail(fmt("%s: %s belongs to another context", op, what));
+  if (b->len < bytes)
+    shape_fail(fmt("%s: %s has %llu bytes, needs %llu", op, what, (unsigned long long)b->len,
+                   (unsigned long long)bytes));
+  if (reinterpret_cast<uintptr_t>(b->ptr) % align) shape_fail(fmt("%s: %s must be %llu-byte aligned", op, what,
+                                                                  (unsigned long long)align));
+}
+// `out`, of which the call writes `bytes`, against what else it touches.
+void check_apart(const char *op, const char *what, const mdma_buf *out, uint64_t bytes, const mdma_buf *in) {
+  if (in && bytes && in->len && out->ptr < in->ptr + in->len && in->ptr < out->ptr + bytes)
+    shape_fail(fmt("%s: %s overlaps another buffer of the call", op, what));
+}
+
+template <class T>
+T *at(const mdma_buf *b) {
+  return reinterpret_cast<T *>(b->ptr);
+}
+
+KvBooks check_pages(mdma_ctx *ctx, const char *op, const mdma_kv_pages *p) {
+  if (!p) shape_fail(fmt("%s: null pages", op));
+  if (!p->n_layers || !p->n_pages || !p->n_seqs || !p->max_pages) shape_fail(fmt("%s: empty cache", op));
+  if (p->n_seqs > KV_MAX_SEQS) shape_fail(fmt("%s: more than %llu sequences", op, (unsigned long long)KV_MAX_SEQS));
+  if (p->page_len < 16 || p->page_len > 256 || (p->page_len & (p->page_len - 1)))
+    shape_fail(fmt("%s: page_len must be 16, 32, 64, 128 or 256", op));
+  if (!p->kv_width || p->kv_width % 8 || p->kv_width > (1u << 20))
+    shape_fail(fmt("%s: kv_width must be a multiple of 8, at most 2^20", op));
+  // Positions and page ids stay below 2^31 (32-bit arithmetic on them in the kernels).
+  if (p->n_pages > INT32_MAX || p->n_layers > 65535 || p->max_pages > INT32_MAX / p->page_len)
+    fail(MDMA_ERR_SIZE_OVERFLOW, fmt("%s: more pages or layers than 32-bit positions reach", op));
+  const uint64_t pool = times(times(p->n_layers, p->n_pages, op), times(2 * p->page_len, p->kv_width, op), op);
+  check_buf(ctx, op, "k", p->k, pool, 16);
+  check_buf(ctx, op, "v", p->v, pool, 16);
+  check_buf(ctx, op, "table", p->table, times(p->n_seqs, p->max_pages, op) * 4, 4);
+  check_buf(ctx, op, "lens", p->lens, p->n_seqs * 4, 4);
+  check_buf(ctx, op, "refs", p->refs, p->n_pages * 4, 4);
+  KvBooks b;
+  b.k = at<uint16_t>(p->k);
+  b.v = at<uint16_t>(p->v);
+  b.table = at<uint32_t>(p->table);
+  b.lens = at<uint32_t>(p->lens);
+  b.refs = at<uint32_t>(p->refs);
+  b.n_layers = (uint32_t)p->n_layers;
+  b.n_pages = (uint32_t)p->n_pages;
+  b.page_shift = (uint32_t)__builtin_ctzll(p->page_len);
+  b.width = (uint32_t)p->kv_width;
+  b.n_seqs = (uint32_t)p->n_seqs;
+  b.max_pages = (uint32_t)p->max_pages;
+  return b;
+}
+// The parts of a cache that a call writes, apart from each other and from `others`.
+void check_books_apart(const char *op, const mdma_kv_pages *p, std::initializer_list<const mdma_buf *> others) {
+  const mdma_buf *mine[5] = {p->k, p->v, p->table, p->lens, p->refs};
+  for (int i = 0; i < 5; i++) {
+    for (int j = 0; j < i; j++) check_apart(op, "a part of the cache", mine[i], mine[i]->len, mine[j]);
+    for (const mdma_buf *o : others) check_apart(op, "the cache", mine[i], mine[i]->len, o);
+  }
+}
+
+PagedView view_of(const KvBooks &b, uint64_t layer, const char *op) {
+  if (layer >= b.n_layers) shape_fail(fmt("%s: layer %llu of %u", op, (unsigned long long)layer, b.n_layers));
+  const uint64_t off = (layer * b.n_pages << b.page_shift) * b.width;
+  return PagedView{b.k + off, b.v + off, b.table, b.lens, nullptr, b.n_pages, b.page_shift, b.width, b.n_seqs,
+                   b.max_pages, 0};
+}
+
+// f32 elements of a [n_seqs][n_new][row] buffer: its n_new.
+uint64_t new_tokens(const char *op, const char *what, const mdma_buf *b, uint64_t n_seqs, uint64_t row) {
+  if (!b) shape_fail(fmt("%s: null %s", op, what));
+  const uint64_t per = times(n_seqs, row, op) * 4;
+  if (!b->len || b->len % per)
+    shape_fail(fmt("%s: %s has %llu bytes, not whole tokens of %llu sequences", op, what, (unsigned long long)b->len,
+                   (unsigned long long)n_seqs));
+  return b->len / per;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mdma_gfx950_kv_pages_fork(mdma_ctx *ctx, const mdma_kv_pages *pages, const mdma_buf *from, const mdma_buf *keep) {
+  return guarded([&] {
+    const char *op = "kv_pages_fork";
+    if (!ctx) shape_fail("kv_pages_fork: null context");
+    std::lock_guard<std::recursive_mutex> g(ctx->lock);
+    const KvBooks b = check_pages(ctx, op, pages);
+    check_buf(ctx, op, "from", from, b.n_seqs * 4ull, 4);
+    if (keep) check_buf(ctx, op, "keep", keep, b.n_seqs * 4ull, 4);
+    check_books_apart(op, pages, {from, keep});
+    OnDevice dev(ctx);
+    q8_invalidate(ctx);
+    auto *tmp = reinterpret_cast<uint32_t *>(scratch(ctx, kv_fork_scratch(b.n_seqs, b.max_pages)));
+    launch_kv_fork(ctx, b, at<const uint32_t>(from), keep ? at<const uint32_t>(keep) : nullptr, tmp);
+  });
+}
+
+int mdma_gfx950_kv_pages_grow(mdma_ctx *ctx, const mdma_kv_pages *pages, const mdma_buf *grow, mdma_buf *status) {
+  return guarded([&] {
+    const char *op = "kv_pages_grow";
+    if (!ctx) shape_fail("kv_pages_grow: null context");
+    std::lock_guard<std::recursive_mutex> g(ctx->lock);
+    const KvBooks b = check_pages(ctx, op, pages);
+    check_buf(ctx, op, "grow", grow, b.n_seqs * 4ull, 4);
+    check_buf(ctx, op, "status", status, b.n_seqs * 4ull, 4);
+    check_books_apart(op, pages, {grow, status});
+    check_apart(op, "status", status, b.n_seqs * 4ull, grow);
+    OnDevice dev(ctx);
+    q8_invalidate(ctx);
+    auto *tmp = reinterpret_cast<uint32_t *>(scratch(ctx, kv_grow_scratch(b.n_seqs, b.n_pages)));
+    launch_kv_grow(ctx, b, at<const uint32_t>(grow), tmp, at<uint32_t>(status));
+  });
+}
+
+int mdma_gfx950_kv_pages_compact(mdma_ctx *ctx, const mdma_kv_pages *pages, mdma_buf *n_live) {
+  return guarded([&] {
+    const char *op = "kv_pages_compact";
+    if (!ctx) shape_fail("kv_pages_compact: null context");
+    std::lock_guard<std::recursive_mutex> g(ctx->lock);
+    const KvBooks b = check_pages(ctx, op, pages);
+    if (n_live) check_buf(ctx, op, "n_live", n_live, 4, 4);
+    check_books_apart(op, pages, {n_live});
+    OnDevice dev(ctx);
+    q8_invalidate(ctx);
+    auto *tmp = reinterpret_cast<uint32_t *>(scratch(ctx, kv_compact_scratch(b.n_pages)));
+    launch_kv_compact(ctx, b, tmp, n_live ? at<uint32_t>(n_live) : nullptr);
+  });
+}
+
+int mdma_gfx950_rope_kv_write_paged(mdma_ctx *ctx, mdma_buf *q, const mdma_buf *k, const mdma_buf *v,
+                                    const mdma_kv_pages *pages, uint64_t layer, const mdma_rope_spec *spec) {
+  return guarded([&] {
+    const char *op = "rope_kv_write_paged";
+    if (!ctx) shape_fail("rope_kv_write_paged: null context");
+    if (!spec) shape_fail("rope_kv_write_paged: null spec");
+    std::lock_guard<std::recursive_mutex> g(ctx->lock);
+    const KvBooks b = check_pages(ctx, op, pages);
+    const PagedView kv = view_of(b, layer, op);
+    const uint64_t hd = spec->head_dim;
+    if (!hd || hd % 2 || b.width % hd) shape_fail("rope_kv_write_paged: kv_width is not whole even heads");
+    if (!std::isfinite(spec->theta) || spec->theta <= 0.f) shape_fail("rope_kv_write_paged: theta must be positive");
+    const uint64_t n_new = new_tokens(op, "k", k, b.n_seqs, b.width), rows = n_new * b.n_seqs;
+    check_buf(ctx, op, "k", k, rows * b.width * 4, 16);
+    check_buf(ctx, op, "v", v, rows * b.width * 4, 16);
+    if (!q || !q->len || q->len % times(rows, hd * 4, op))
+      shape_fail("rope_kv_write_paged: q is not whole heads of k's tokens");
+    check_buf(ctx, op, "q", q, q->len, 16);
+    const uint64_t q_heads = q->len / (rows * hd * 4);
+    if (rows > INT32_MAX || q_heads * hd > (1u << 24)) fail(MDMA_ERR_SIZE_OVERFLOW, "rope_kv_write_paged: too many rows");
+    check_books_apart(op, pages, {q, k, v});
+    check_apart(op, "q", q, q->len, k);
+    check_apart(op, "q", q, q->len, v);
+    OnDevice dev(ctx);
+    q8_invalidate(ctx);
+    const float *tab = rope_table(ctx, ((uint64_t)b.max_pages << b.page_shift) - 1, hd, spec->theta);
+    launch_rope_kv_paged(ctx, at<float>(q), at<const float>(k), at<const float>(v), kv, (uint32_t)n_new,
+                         (uint32_t)q_heads, (uint32_t)(b.width / hd), (uint32_t)hd, tab);
+  });
+}
+
+int mdma_gfx950_attn_paged(mdma_ctx *ctx, const mdma_buf *q, const mdma_kv_pages *pages, uint64_t layer,
+                           const mdma_buf *prefix, const mdma_attn_spec *spec, mdma_buf *o) {
+  return guarded([&] {
+    const char *op = "attn_paged";
+    if (!ctx) shape_fail("attn_paged: null context");
+    if (!spec) shape_fail("attn_paged: null spec");
+    std::lock_guard<std::recursive_mutex> g(ctx->lock);
+    const KvBooks b = check_pages(ctx, op, pages);
+    PagedView kv = view_of(b, layer, op);
+    const uint64_t hd = spec->head_dim, H = spec->n_q_heads, KV = spec->n_kv_heads;
+    if (!hd || hd % 8 || hd > 256) shape_fail("attn_paged: head_dim must be a multiple of 8, at most 256");
+    if (!KV || KV > b.width || KV * hd != b.width) shape_fail("attn_paged: n_kv_heads * head_dim is not kv_width");
+    if (!H || H > 65535 || H % KV) shape_fail("attn_paged: q heads are not a multiple of KV heads");
+    const uint64_t n_new = new_tokens(op, "q", q, b.n_seqs, H * hd), bytes = q->len;
+    if (n_new * b.n_seqs * H > INT32_MAX) fail(MDMA_ERR_SIZE_OVERFLOW, "attn_paged: too many query rows");
+    check_buf(ctx, op, "q", q, bytes, 16);
+    check_buf(ctx, op, "o", o, bytes, 16);
+    if (prefix) {
+      check_buf(ctx, op, "prefix", prefix, 0, 4);
+      if (prefix->len % 4 || prefix->len / 4 > b.max_pages)
+        shape_fail("attn_paged: prefix is not whole page ids, at most max_pages");
+      kv.prefix = at<const uint32_t>(prefix);
+      kv.n_prefix = (uint32_t)(prefix->len / 4);
+    }
+    for (const mdma_buf *x : {(const mdma_buf *)pages->k, (const mdma_buf *)pages->v, (const mdma_buf *)pages->table,
+                              (const mdma_buf *)pages->lens, (const mdma_buf *)pages->refs, q, prefix})
+      check_apart(op, "o", o, bytes, x);
+    OnDevice dev(ctx);
+    q8_invalidate(ctx);
+    q8_invalidate_range(ctx, o->ptr, bytes);
+    launch_attn_paged(ctx, at<const float>(q), kv, (uint32_t)n_new, (uint32_t)H, (uint32_t)KV, (uint32_t)hd,
+                      at<float>(o));
+  });
+}
+
+int mdma_gfx950_lora_new(mdma_ctx *ctx, int32_t dtype, uint64_t n_in, uint64_t n_out, uint64_t max_rank,
+                         uint64_t n_slots, mdma_lora **out) {
+  return guarded([&] {
+    const char *op = "lora_new";
+    if (!ctx || !out) shape_fail("lora_new: null argument");
+    *out = nullptr;
+    if (dtype != DT_F32 && dtype != DT_F16) fail(MDMA_ERR_NOT_IMPLEMENTED, fmt("lora_new: dtype %d", dtype));
+    if (!n_in || !n_out || !max_rank || !n_slots) shape_fail("lora_new: empty adapters");
+    if (max_rank > 256) shape_fail("lora_new: max_rank above 256");
+    if (n_in > (1u << 24) || n_out > (1u << 24) || n_slots > 65536)
+      fail(MDMA_ERR_SIZE_OVERFLOW, "lora_new: more than 2^24 columns or rows, or 65536 slots");
+    std::lock_guard<std::recursive_mutex> g(ctx->lock);
+    OnDevice dev(ctx);
+    auto l = std::make_unique<mdma_lora>();
+    l->ctx = ctx;
+    l->max_rank = max_rank;
+    const uint64_t eb = type_size(dtype), rp = (max_rank + 15) / 16 * 16, ip = (n_in + 31) / 32 * 32;
+    auto take = [&](uint64_t bytes, mdma_buf **b) {
+      const int st = mdma_gfx950_alloc(ctx, bytes, MDMA_POOL_WEIGHTS, b);
+      if (st) fail(st, mdma_gfx950_last_error());
+    };
+    take(times(n_slots, rp * ip * eb, op), &l->a);
+    take(times(n_slots, n_out * rp * eb, op), &l->b);
+    take(n_slots * sizeof(LoraSlot), &l->info);
+    const std::vector<LoraSlot> none(n_slots);
+    const int st = mdma_gfx950_upload(ctx, l->info, 0, none.data(), n_slots * sizeof(LoraSlot));
+    if (st) fail(st, mdma_gfx950_last_error());
+    l->view = LoraView{dtype, (uint32_t)n_in, (uint32_t)n_out, (uint32_t)ip, (uint32_t)rp, (uint32_t)n_slots,
+                       l->a->ptr, l->b->ptr, reinterpret_cast<const LoraSlot *>(l->info->ptr)};
+    *out = l.release();
+  });
+}
+
+int mdma_gfx950_lora_load(mdma_lora *l, uint64_t slot, const void *a, const void *b, uint64_t rank, float scale) {
+  return guarded([&] {
+    if (!l || (rank && (!a || !b))) shape_fail("lora_load: null argument");
+    const LoraView &w = l->view;
+    if (slot >= w.n_slots) shape_fail("lora_load: no such slot");
+    if (rank > l->max_rank) shape_fail("lora_load: rank above max_rank");
+    std::lock_guard<std::recursive_mutex> g(l->ctx->lock);
+    OnDevice dev(l->ctx);
+    const uint64_t eb = type_size(w.dtype), stride = (rank + 15) / 16 * 16;
+    // Rows padded with zeros: columns to in_pad, ranks to whole 16s.
+    std::vector<char> pa(stride * w.in_pad * eb), pb(w.n_out * stride * eb);
+    for (uint64_t r = 0; r < rank; r++)
+      memcpy(&pa[r * w.in_pad * eb], static_cast<const char *>(a) + r * w.n_in * eb, w.n_in * eb);
+    for (uint64_t n = 0; rank && n < w.n_out; n++)
+      memcpy(&pb[n * stride * eb], static_cast<const char *>(b) + n * rank * eb, rank * eb);
+    const LoraSlot in{(uint32_t)rank, (uint32_t)stride, scale};
+    auto put = [&](mdma_buf *dst, uint64_t off, const void *src, uint64_t n) {
+      const int st = mdma_gfx950_upload(l->ctx, dst, off, src, n);
+      if (st) fail(st, mdma_gfx950_last_error());
+    };
+    // (An upload waits for the stream: calls queued before read the slot as it was.)
+    put(l->a, slot * w.rank_pad * w.in_pad * eb, pa.data(), pa.size());
+    put(l->b, slot * w.n_out * w.rank_pad * eb, pb.data(), pb.size());
+    put(l->info, slot * sizeof(LoraSlot), &in, sizeof in);
+  });
+}
+
+int mdma_gfx950_lora_add(mdma_ctx *ctx, const mdma_lora *l, const mdma_buf *ids, const mdma_buf *x,
+                         const mdma_buf *base, mdma_buf *y) {
+  return guarded([&] {
+    const char *op = "lora_add";
+    if (!ctx || !l) shape_fail("lora_add: null argument");
+    if (l->ctx != ctx) shape_fail("lora_add: adapters belong to another context");
+    std::lock_guard<std::recursive_mutex> g(ctx->lock);
+    const LoraView &w = l->view;
+    const uint64_t T = new_tokens(op, "x", x, 1, w.n_in);
+    if (T > (1u << 24)) fail(MDMA_ERR_SIZE_OVERFLOW, "lora_add: more than 2^24 tokens");
+    const uint64_t out = T * w.n_out * 4;
+    check_buf(ctx, op, "x", x, x->len, 16);
+    check_buf(ctx, op, "ids", ids, T * 4, 4);
+    check_buf(ctx, op, "base", base, out, 16);
+    check_buf(ctx, op, "y", y, out, 16);
+    check_apart(op, "y", y, out, x);
+    check_apart(op, "y", y, out, ids);
+    for (const mdma_buf *own : {l->a, l->b, l->info}) check_apart(op, "y", y, out, own);
+    if (y->ptr != base->ptr) check_apart(op, "y", y, out, base);
+    OnDevice dev(ctx);
+    q8_invalidate(ctx);
+    q8_invalidate_range(ctx, y->ptr, out);
+    float *u = reinterpret_cast<float *>(scratch(ctx, lora_scratch(w, T)));
+    launch_lora(ctx, w, at<const uint32_t>(ids), (uint32_t)T, at<const float>(x), at<const float>(base), at<float>(y),
+                u);
+  });
+}
+
+int mdma_gfx950_lora_free(mdma_lora *l) {
+  return guarded([&] {
+    if (!l) return;
+    std::lock_guard<std::recursive_mutex> g(l->ctx->lock);
+    if (l->ctx->capturing) fail(MDMA_ERR_BACKEND, "lora_free: synchronizes and cannot run under graph capture");
+    OnDevice dev(l->ctx);
+    delete l;
+  });
+}
+
+}  // extern "C"
