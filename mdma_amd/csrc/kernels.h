@@ -206,6 +206,24 @@ __device__ __forceinline__ float wave_sum_all(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
+// Max / sum over the lanes l, l ^ 16, l ^ 32, l ^ 48, in every one of them.
+__device__ __forceinline__ float quarter_max(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const float w = fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+  const uint32_t x = __builtin_bit_cast(uint32_t, w);
+  const auto c = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)c[0]), __builtin_bit_cast(float, (uint32_t)c[1]));
+}
+__device__ __forceinline__ float quarter_sum(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const float w = __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
+  const uint32_t x = __builtin_bit_cast(uint32_t, w);
+  const auto c = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return __builtin_bit_cast(float, (uint32_t)c[0]) + __builtin_bit_cast(float, (uint32_t)c[1]);
+}
+
 // Six-bit (scale, min) of Q4_K sub-blocks 2p and 2p+1 from the header's
 // 12 scale bytes (hd.y, hd.z, hd.w): get_scale_min_k4 of
 // /root/reference/src/backend/rocm/kernels/kernels.hip:19-27, evaluated for

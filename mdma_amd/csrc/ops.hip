@@ -511,24 +511,6 @@ typedef float v4f_t __attribute__((ext_vector_type(4)));
 typedef _Float16 v4h_t __attribute__((ext_vector_type(4)));
 typedef float v4f_u __attribute__((ext_vector_type(4), aligned(4)));
 
-// Max / sum over the lanes l, l ^ 16, l ^ 32, l ^ 48, in every one of them.
-__device__ __forceinline__ float quarter_max(float v) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, v);
-  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const float w = fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
-  const uint32_t x = __builtin_bit_cast(uint32_t, w);
-  const auto c = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  return fmaxf(__builtin_bit_cast(float, (uint32_t)c[0]), __builtin_bit_cast(float, (uint32_t)c[1]));
-}
-__device__ __forceinline__ float quarter_sum(float v) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, v);
-  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const float w = __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
-  const uint32_t x = __builtin_bit_cast(uint32_t, w);
-  const auto c = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  return __builtin_bit_cast(float, (uint32_t)c[0]) + __builtin_bit_cast(float, (uint32_t)c[1]);
-}
-
 template <int G, int HD>
 __global__ __launch_bounds__(256) void attn_prefill_kernel(const float *__restrict__ q, const uint16_t *__restrict__ K,
                                                            const uint16_t *__restrict__ V, float *__restrict__ o,
