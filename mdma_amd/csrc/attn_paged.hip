@@ -19,6 +19,8 @@
 //    p, and 2^-35 of the row's largest p.
 // m is a whole number, so 2^(m - m') is a power of two: rescaling l and O
 // and joining chunks round nothing.
+#include <type_traits>
+
 #include "kernels.h"
 #include "paged.h"
 
@@ -66,23 +68,51 @@ __device__ __forceinline__ uint32_t seen_by(uint32_t len, uint32_t n_new, uint32
   return len + j + 1 > n_new ? len + j + 1 - n_new : 0;
 }
 
-// LDS slot of 16-byte chunk ch of a key's row of KC chunks: keys read together
-// (16 rows of one chunk; 4 rows of a 32-byte column by a transposing read) fall on
+// A 16-key block of K or V in LDS: KC 16-byte chunks a key, 1024 bytes a
+// DMA instruction. Instruction i of a lane brings the chunk that belongs at
+// 1024 i + 16 lane. KC a power of two: keys in rows of KC chunks, so an
+// instruction reads whole rows of memory (16 lanes a 256-byte row: of 64 bytes a row,
+// every 128-byte line is looked up twice, and the loads of a tile took twice as long),
+// chunk ch of key k in slot ch ^ f(k). KC = 12: four chunks of 16 keys an instruction. Either
+// way the reads below, 16 rows of one chunk or 4 rows of a 32-byte column at a time, meet
 // different banks.
 template <int KC>
-__device__ __forceinline__ uint32_t slot_of(uint32_t key, uint32_t ch) {
-  if constexpr (KC == 8) return ch ^ ((key >> 1) & 7);
-  else if constexpr (KC == 12) {
-    const uint32_t s = ch + (key & 15) / 2;
-    return s >= KC ? s - KC : s;
-  } else return ch ^ (key & 15);
+__device__ __forceinline__ uint32_t mix(uint32_t key) {
+  return KC == 8 ? (key >> 1) & 7 : KC == 12 ? 2 * (key >> 2 & 1) : key & 15;
 }
-// Byte offset of chunk ch + step of a key's row, `at` that of chunk ch (ch <
-// the power of two step): an XOR away where slot_of is one.
 template <int KC>
-__device__ __forceinline__ uint32_t chunk_on(uint32_t at, uint32_t key, uint32_t ch, int step) {
-  if constexpr (KC == 12) return (key * KC + slot_of<KC>(key, ch + step)) * 16;
+__device__ __forceinline__ uint32_t lds_of(uint32_t key, uint32_t ch) {
+  if constexpr (KC == 12) return 1024 * (ch >> 2) + 64 * key + 16 * ((ch & 3) ^ mix<KC>(key));
+  else return (key * KC + (ch ^ mix<KC>(key))) * 16;
+}
+// lds_of chunk ch + step from `at`, that of ch (ch < 4, step a multiple of 4; ch < 2, of 2).
+template <int KC>
+__device__ __forceinline__ uint32_t chunk_on(uint32_t at, int step) {
+  if constexpr (KC == 12) return (at ^ (16 * (step & 3))) + 1024 * (step >> 2);
   else return at ^ (16 * step);
+}
+// The key and chunk that lane `lane` brings with instruction i.
+template <int KC>
+__device__ __forceinline__ uint32_t dma_key(uint32_t lane, int i) {
+  return KC == 12 ? lane >> 2 : (64 / KC) * i + lane / KC;
+}
+template <int KC>
+__device__ __forceinline__ uint32_t dma_chunk(uint32_t lane, int i) {
+  return KC == 12 ? 4 * i + ((lane & 3) ^ mix<KC>(lane >> 2)) : (lane % KC) ^ mix<KC>(dma_key<KC>(lane, i));
+}
+template <int N>
+__device__ __forceinline__ void wait_dma() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// Least / most of a row of 16 lanes, in all of them.
+template <bool MOST>
+__device__ __forceinline__ uint32_t row16(uint32_t v) {
+  auto f = [](uint32_t x, uint32_t y) { return MOST ? max(x, y) : min(x, y); };
+  v = f(v, dpp_u32<0xB1, 0xF>(v));
+  v = f(v, dpp_u32<0x4E, 0xF>(v));
+  v = f(v, dpp_u32<0x141, 0xF>(v));
+  return f(v, dpp_u32<0x140, 0xF>(v));
 }
 // A value the compiler takes as new here: what is cheap to derive from it
 // is derived again in every tile, not kept in registers over the loop.
@@ -153,21 +183,22 @@ __device__ __forceinline__ void row_by_keys(const Args &a, const Job &job, uint3
   *l_out = wave_sum_all(l);
 }
 
-// Jobs come in two kinds. Narrow: up to 64 query rows, 16 a wave; where
+// K and V come to LDS by DMA, in flight over the arithmetic and in no
+// registers. Jobs come in two kinds. Narrow: up to 64 query rows, 16 a wave; where
 // they are fewer than the workgroup's four waves hold, the waves of one row block take
-// 32-key tiles in turn. K comes straight from memory as MFMA operands, V
-// through 32 keys of LDS of the wave's own (ds_read_b64_tr_b16 gives
-// its columns), no barrier until the waves join at the end. Wide: 64 MB rows,
-// 16 MB a wave; the waves share 64-key tiles of K and V in two LDS buffers,
+// 32-key tiles in turn. Each wave has LDS of its own for a tile of K and one of V; the next K is
+// asked for when the products with the last are done, the next V when its columns
+// (ds_read_b64_tr_b16) are read; no barrier until the waves join at the end. Wide: 64 MB
+// rows, 16 MB a wave; the waves share 64-key tiles of K and V in two LDS buffers,
 // one barrier a tile. NC: head_dim in 32s, rounded up; the dims past head_dim
 // read some other dim of the same key with q 0 there. WIDE: whether there are
 // wide jobs.
 template <int NC, int MB, bool WIDE>
 __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a) {
   constexpr int KC = 4 * NC, ND = 2 * NC, NA = (NC + 1) / 2;
-  __shared__ __attribute__((aligned(16))) char lds[(WIDE ? 16 : 8) * 1024 * NC];
+  __shared__ __attribute__((aligned(16))) char lds[16 * 1024 * NC];
   __shared__ float2 ml[4][16];
-  __shared__ uint32_t flags[4];
+  __shared__ uint32_t most[4];
   const uint32_t tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lq = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -259,17 +290,6 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
         lo[i >> 1][4 * (i & 1) + e] = w[0], lo[i >> 1][4 * (i & 1) + e + 1] = w[1];
       }
   };
-  // The least and the most that the wave's rows see.
-  auto spread = [&](uint32_t &least, uint32_t &most) __attribute__((always_inline)) {
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) {
-      least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
-      most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
-    }
-    least = __builtin_amdgcn_readfirstlane(least);
-    most = __builtin_amdgcn_readfirstlane(most);
-  };
-
   // ---- page ids: lane i holds that of 16-key block id0 + i of the part ----
   uint32_t idv, id0 = 0;
   bool holes = false;  // a block met so far has no page
@@ -338,24 +358,33 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
       }
     l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
   };
-  // V's columns of 32 keys (rows of KC chunks in LDS from `v`) for dims 16 n, from those of dims 0.
-  const uint32_t v_key = 4 * lq + (l16 >> 2), v_ch = (l16 & 3) >> 1;
-  const uint32_t v_at = (v_key * KC + slot_of<KC>(v_key, v_ch)) * 16 + 8 * (l16 & 1);
+  // V's columns of 32 keys (two blocks in LDS from `v`) for dims 16 n, from those of dims 0.
+  const uint32_t k_at = lds_of<KC>(l16, lq);
+  const uint32_t v_at = lds_of<KC>(4 * lq + (l16 >> 2), (l16 & 3) >> 1) + 8 * (l16 & 1);
   auto v_columns = [&](const char *v, uint32_t at0, int n) __attribute__((always_inline)) {
-    uint32_t at = chunk_on<KC>(at0, v_key, v_ch, 2 * n);
-    if (KC == 12) at += 8 * (l16 & 1);
-    auto rd = [&](uint32_t x) {
+    auto rd = [&](const char *x) {
       return __builtin_bit_cast(v4h_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                           (__attribute__((address_space(3))) v4s_t *)(v + x)));
+                                           (__attribute__((address_space(3))) v4s_t *)x));
     };
-    const v4h_t x = rd(at), y = rd(at + 16 * KC * 16);  // (slot_of has period 16 in the key)
+    const char *at = v + chunk_on<KC>(at0, 2 * n);
+    const v4h_t x = rd(at), y = rd(at + 1024 * NC);
     return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  // Where this lane puts its chunks of a 16-key block: key lane / 4, chunks lane % 4 + 4 i; and reads them.
-  const uint32_t w_key = lane >> 2, w_ch = lane & 3, w_at = (w_key * KC + slot_of<KC>(w_key, w_ch)) * 16;
   uint32_t row_off[NC];
 #pragma unroll
-  for (int i = 0; i < NC; i++) row_off[i] = w_key * row_bytes + 16 * min(4 * i + w_ch, last_ch);
+  for (int i = 0; i < NC; i++)
+    row_off[i] = dma_key<KC>(lane, i) * row_bytes + 16 * min(dma_chunk<KC>(lane, i), last_ch);
+  // One 16-key block at byte `at` of a pool into LDS.
+  auto dma = [&](const char *pool, uint64_t at, const char *to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NC; i++) lds_dma16(pool + at, row_off[i], to + 1024 * i);
+  };
+  // Rows past the end hold anything: 0 of it is to be 0. (left: keys of the block before the end)
+  auto clear_rows = [&](char *v, int left) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NC; i++)
+      if ((int)dma_key<KC>(lane, i) >= left) *reinterpret_cast<u32x4 *>(v + 1024 * i + 16 * lane) = u32x4{0, 0, 0, 0};
+  };
   float *part_o = a.part;
   float2 *part_ml = reinterpret_cast<float2 *>(a.part + (uint64_t)(a.n_p + a.n_t) * a.rows * a.hd);
   auto out_row = [&](const Row &x) __attribute__((always_inline)) {
@@ -383,34 +412,25 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
     // Wave w: row block w % rb, of each 128 keys every (4 / rb)-th 32.
     const uint32_t rs = job.n_rows <= 16 ? 0 : job.n_rows <= 32 ? 1 : 2, rb = 1 << rs, per = 4 >> rs;
     const uint32_t mine = wave & (rb - 1), turn = wave >> rs;
+    fetch_ids();
     const Row row = row_of(16 * mine + l16);
     v4f_t qv[2 * NC];
     load_q(row, qv);
-    fetch_ids();
-    uint32_t seen_max = row.seen, seen_min = row.seen;
-    spread(seen_min, seen_max);
+    const uint32_t seen_max = __builtin_amdgcn_readfirstlane(row16<true>(row.seen));
+    const uint32_t seen_min = __builtin_amdgcn_readfirstlane(row16<false>(row.seen));
     const uint32_t end = min(job.k0 + job.n, seen_max);
-    note_holes();
-    char *vs = lds + wave * (32 * KC * 16);
-    uint32_t k_off[NC];
-#pragma unroll
-    for (int i = 0; i < NC; i++) k_off[i] = l16 * row_bytes + 16 * min(4 * i + lq, last_ch);
-    u32x4 kr[2][NC], vr[2][NC];
+    char *ks = lds + wave * (4096 * NC), *vs = ks + 2048 * NC;
     auto block_of = [&](uint32_t it) __attribute__((always_inline)) { return 8 * (it >> rs) + 2 * ((it & (rb - 1)) * per + turn); };
-    auto gload = [&](uint32_t block) __attribute__((always_inline)) {
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++) {
-        const uint64_t at = block_at(block + kb);
-        const char *K = Kh + at, *V = Vh + at;
-#pragma unroll
-        for (int i = 0; i < NC; i++) kr[kb][i] = *reinterpret_cast<const u32x4 *>(K + k_off[i]);
-#pragma unroll
-        for (int i = 0; i < NC; i++) vr[kb][i] = *reinterpret_cast<const u32x4 *>(V + row_off[i]);
-      }
-    };
     uint32_t it = 0, block = block_of(0), pos = job.at(block);
-    if (pos < end) gload(block);
-    __builtin_amdgcn_sched_barrier(0);
+    uint64_t at0 = 0, at1 = 0;
+    note_holes();
+#pragma unroll
+    for (int i = 0; i < 2 * NC; i++) asm volatile("" : "+v"(qv[i]));  // (arrived, before loads the compiler does not count)
+    if (pos < end) {
+      at0 = block_at(block), at1 = block_at(block + 1);
+      dma(Kh, at0, ks), dma(Kh, at1, ks + 1024 * NC);
+      dma(Vh, at0, vs), dma(Vh, at1, vs + 1024 * NC);
+    }
     v8h_t qh[NC], ql[NC];
     float c, m = -INFINITY, l = 0.f;
     v4f_t O[ND];
@@ -418,19 +438,7 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
 #pragma unroll
     for (int n = 0; n < ND; n++) O[n] = v4f_t{0.f, 0.f, 0.f, 0.f};
     while (pos < end) {
-      if (pos + 32 > end) {  // (uniform) rows past the end hold anything: 0 of it is to be 0
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-          if (pos + 16 * kb + w_key >= end) {
-#pragma unroll
-            for (int i = 0; i < NC; i++) vr[kb][i] = u32x4{0, 0, 0, 0};
-          }
-      }
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-        for (int i = 0; i < NC; i++)
-          *reinterpret_cast<u32x4 *>(vs + 16 * kb * KC * 16 + chunk_on<KC>(w_at, w_key, w_ch, 4 * i)) = vr[kb][i];
+      wait_dma<2 * NC>();  // K is there (V was asked for after it)
       // (four sums, so that no product waits for the last one: q's low parts apart)
       const v4f_t zero = {0.f, 0.f, 0.f, 0.f};
       v4f_t S[2], Sl[2];
@@ -438,72 +446,92 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
       for (int j = 0; j < NC; j++)
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
-          const v8h_t K = __builtin_bit_cast(v8h_t, kr[kb][j]);
+          const v8h_t K = *reinterpret_cast<const v8h_t *>(ks + 1024 * NC * kb + chunk_on<KC>(k_at, 4 * j));
           Sl[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K, ql[j], j ? Sl[kb] : zero, 0, 0, 0);
           S[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K, qh[j], j ? S[kb] : zero, 0, 0, 0);
         }
       const uint32_t now = pos, now_block = block;
       const bool mask = now + 32 > seen_min || holes;
-      it++;
-      const uint32_t next = block_of(it);
-      pos = job.at(next);
-      block = pos < end ? next : now_block;  // (past the end: this tile again, unused)
-      __builtin_amdgcn_sched_barrier(0);
-      gload(block);  // in flight over the rest of this tile
-      __builtin_amdgcn_sched_barrier(0);
-      v8h_t V[ND], Ph, Pl;  // (V under way over the softmax)
-#pragma unroll
-      for (int n = 0; n < ND; n++) V[n] = v_columns(vs, v_at, n);
+      block = block_of(++it);
+      pos = job.at(block);
+      const bool more = pos < end;
+      wait_lds();
+      if (more) {
+        at0 = block_at(block), at1 = block_at(block + 1);
+        dma(Kh, at0, ks), dma(Kh, at1, ks + 1024 * NC);
+      }
 #pragma unroll
       for (int kb = 0; kb < 2; kb++) S[kb] += Sl[kb];
+      v8h_t V[ND], Ph, Pl;
       weights(S, c, row.seen, mask, now, now_block, m, l, O, Ph, Pl);
+      if (more) wait_dma<2 * NC>();  // V is there
+      else wait_dma<0>();
+      if (now + 32 > end) {  // (uniform)
+        clear_rows(vs, (int)(end - now));
+        clear_rows(vs + 1024 * NC, (int)(end - now) - 16);
+      }
+#pragma unroll
+      for (int n = 0; n < ND; n++) V[n] = v_columns(vs, v_at, n);
+      wait_lds();
+      if (more) dma(Vh, at0, vs), dma(Vh, at1, vs + 1024 * NC);
 #pragma unroll
       for (int n = 0; n < ND; n++) O[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(V[n], Pl, O[n], 0, 0, 0);
 #pragma unroll
       for (int n = 0; n < ND; n++) O[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(V[n], Ph, O[n], 0, 0, 0);
     }
     // ---- the waves' parts joined: wave w the dims 16 (turn + per b) of its row block ----
-    if (tid < 4) flags[tid] = 0;
     l = quarter_sum(l);
+    float z = l;  // not finite where any value is not, of any lane of the row
+#pragma unroll
+    for (int n = 0; n < ND; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) z = fmaf(O[n][e], 0.f, z);
+    l = quarter_sum(z * 0.f) + l;  // NaN then
     if (lq == 0) ml[wave][l16] = make_float2(m, l);
     v4f_t *ob = reinterpret_cast<v4f_t *>(lds);
-    __syncthreads();  // (all reads of V's tiles are done)
+    __syncthreads();  // (all reads of the tiles are done)
 #pragma unroll
     for (int n = 0; n < ND; n++) ob[(wave * ND + n) * 64 + lane] = O[n];
-    float M = -INFINITY, L = 0.f, w[4];
-#pragma unroll
-    for (int v = 0; v < 4; v++) M = fmaxf(M, v < (int)per ? ml[mine + rb * v][l16].x : -INFINITY);
-#pragma unroll
-    for (int v = 0; v < 4; v++) {
-      const float2 x = v < (int)per ? ml[mine + rb * v][l16] : make_float2(-INFINITY, 0.f);
-      w[v] = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - M);
-      L = fmaf(x.y, w[v], L);
-    }
     __syncthreads();
-    const float by = times(M, L);
-    float *dst = out_row(row) + 4 * lq;
-    float z = 0.f;  // NaN from any value that is not finite
-    for (uint32_t n = turn; n < ND; n += per) {
-      v4f_t R = {0.f, 0.f, 0.f, 0.f};
-      for (uint32_t v = 0; v < per; v++) {
-        const float wv = v == 0 ? w[0] : v == 1 ? w[1] : v == 2 ? w[2] : w[3];
-        R += ob[((mine + rb * v) * ND + n) * 64 + lane] * wv;
+    auto join = [&](auto PER) __attribute__((always_inline)) {
+      constexpr int per = decltype(PER)::value, rb = 4 / per;
+      float M = -INFINITY, L = 0.f, w[per];
+      float2 x[per];
+#pragma unroll
+      for (int v = 0; v < per; v++) {
+        x[v] = ml[mine + rb * v][l16];
+        M = fmaxf(M, x[v].x);
       }
 #pragma unroll
-      for (int e = 0; e < 4; e++) z = fmaf(R[e], 0.f, z);
-      if (row.there && 16 * n + 4 * lq < a.hd)
-        *reinterpret_cast<v4f_t *>(dst + 16 * n) = M == -INFINITY ? v4f_t{0.f, 0.f, 0.f, 0.f} : R * by;
-    }
-    if (turn == 0 && lq == 0 && row.there) put_ml(row, M, L);
-    const bool bad = row.there && row.seen > job.at(0) && (!(fmaf(L, 0.f, z) == 0.f) || M == -INFINITY);
-    const uint64_t all = __ballot(bad);
-    if (all && lane == 0) atomicOr(&flags[mine], (uint32_t)(all | all >> 16 | all >> 32 | all >> 48) & 0xffff);
-    __syncthreads();  // (and the stores above are done: the slow rows' come after them)
-    for (uint32_t b = 0; b < rb; b++)
-      for (uint32_t todo = flags[b]; todo; todo &= todo - 1) {
-        const uint32_t r = __builtin_ctz(todo);
-        if (r % 4 == wave) slow_row(row_of(16 * b + r));
+      for (int v = 0; v < per; v++) {
+        w[v] = x[v].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[v].x - M);
+        L = fmaf(x[v].y, w[v], L);
       }
+      const bool none = M == -INFINITY, bad = row.there && row.seen > job.at(0) && (none || !(L * 0.f == 0.f));
+      const float by = times(M, L);
+      float *dst = out_row(row) + 4 * lq;
+#pragma unroll
+      for (int b = 0; b < (ND + per - 1) / per; b++) {
+        const uint32_t n = turn + per * b;
+        if (n >= ND) break;
+        v4f_t R = ob[(mine * ND + n) * 64 + lane] * w[0];
+#pragma unroll
+        for (int v = 1; v < per; v++) R += ob[((mine + rb * v) * ND + n) * 64 + lane] * w[v];
+        if (row.there && !bad && 16 * n + 4 * lq < a.hd)
+          *reinterpret_cast<v4f_t *>(dst + 16 * n) = none ? v4f_t{0.f, 0.f, 0.f, 0.f} : R * by;
+      }
+      if (turn == 0 && lq == 0 && row.there && !bad) put_ml(row, M, L);
+      // (every wave of the row block finds the same rows; each takes some)
+      uint32_t todo = (uint32_t)__ballot(bad) & 0xffff;
+#pragma unroll 1
+      for (; todo; todo &= todo - 1) {
+        const uint32_t r = __builtin_ctz(todo);
+        if (r % per == turn) slow_row(row_of(16 * mine + r));
+      }
+    };
+    if (rs == 0) join(std::integral_constant<int, 4>());
+    else if (rs == 1) join(std::integral_constant<int, 2>());
+    else join(std::integral_constant<int, 1>());
     return;
   }
 
@@ -528,66 +556,48 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
       seen_max = max(seen_max, row[i].seen);
       seen_min = min(seen_min, row[i].seen);
     }
-    spread(seen_min, seen_max);
+    seen_max = __builtin_amdgcn_readfirstlane(row16<true>(seen_max));
+    seen_min = __builtin_amdgcn_readfirstlane(row16<false>(seen_min));
     note_holes();
-    if (lane == 0) flags[wave] = seen_max;
+    if (lane == 0) most[wave] = seen_max;
     __syncthreads();
-    const uint32_t end = min(job.k0 + job.n, max(max(flags[0], flags[1]), max(flags[2], flags[3])));
-    // 64-key tiles, two in each 128-key block of the part.
+    const uint32_t end = min(job.k0 + job.n, max(max(most[0], most[1]), max(most[2], most[3])));
+    // 64-key tiles, two in each 128-key block of the part; wave w brings the tile's 16-key block w.
     auto tile_at = [&](uint32_t t) __attribute__((always_inline)) { return job.at(4 * t); };
-    u32x4 kr[NC], vr[NC];
-    // Wave w brings the tile's 16-key block w.
-    auto gload = [&](uint32_t t) __attribute__((always_inline)) {
+    constexpr uint32_t TILE = 4096 * NC;  // bytes of a K or a V tile
+    auto bring = [&](uint32_t t) __attribute__((always_inline)) {
       const uint64_t at = block_at(4 * t + wave);
-#pragma unroll
-      for (int i = 0; i < NC; i++) {
-        kr[i] = *reinterpret_cast<const u32x4 *>(Kh + at + row_off[i]);
-        vr[i] = *reinterpret_cast<const u32x4 *>(Vh + at + row_off[i]);
-      }
+      char *b = lds + (t & 1) * (2 * TILE) + wave * (1024 * NC);
+      dma(Kh, at, b);
+      dma(Vh, at, b + TILE);
     };
-    const uint32_t k_at = (l16 * KC + slot_of<KC>(l16, lq)) * 16;
-    constexpr uint32_t TILE = 64 * KC * 16;  // bytes of a K or a V tile
-    auto to_lds = [&](uint32_t t) __attribute__((always_inline)) {
+    auto arrived = [&](uint32_t t) __attribute__((always_inline)) {
+      wait_dma<0>();
       const uint32_t pos = tile_at(t) + 16 * wave;
-      if (pos + 16 > end && pos + w_key >= end) {  // rows past the end hold anything: 0 of it is to be 0
-#pragma unroll
-        for (int i = 0; i < NC; i++) vr[i] = u32x4{0, 0, 0, 0};
-      }
-      char *b = lds + (t & 1) * (2 * TILE) + 16 * wave * KC * 16;
-      const uint32_t at = anew(w_at);
-#pragma unroll
-      for (int i = 0; i < NC; i++) {
-        const uint32_t off = chunk_on<KC>(at, w_key, w_ch, 4 * i);
-        *reinterpret_cast<u32x4 *>(b + off) = kr[i];
-        *reinterpret_cast<u32x4 *>(b + TILE + off) = vr[i];
-      }
+      if (pos + 16 > end)  // (uniform)
+        clear_rows(lds + (t & 1) * (2 * TILE) + wave * (1024 * NC) + TILE, (int)(end - pos));
     };
-    if (tile_at(0) < end) {
-      gload(0);
-      to_lds(0);
-      if (tile_at(1) < end) gload(1);
-    }
+    if (tile_at(0) < end) bring(0);
     for (uint32_t t = 0; tile_at(t) < end; t++) {
-      lds_barrier();  // tile t is written; the reads of tile t - 1, whose buffer comes next, are done
-      if (tile_at(t + 1) < end) {
-        to_lds(t + 1);
-        if (tile_at(t + 2) < end) gload(t + 2);
-      }
+      arrived(t);
+      lds_barrier();  // tile t is there; the reads of tile t - 1, whose buffer comes next, are done
+      if (tile_at(t + 1) < end) bring(t + 1);
       const uint32_t pos0 = tile_at(t);
       if (pos0 >= seen_max) continue;  // (uniform: none of this wave's rows sees the tile)
-      const char *kb_ = lds + (t & 1) * (2 * TILE);
+      const char *tile = lds + (t & 1) * (2 * TILE);
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const uint32_t pos = pos0 + 32 * half;
         const bool mask = pos + 32 > seen_min || holes;
+        const char *k = tile + 2048 * NC * half;
         v4f_t S[MB][2];
         const uint32_t kat = anew(k_at), vat = anew(v_at);
         // (q's low parts before the high ones)
         const v4f_t zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NC; j++) {
-          const char *k = kb_ + 32 * half * KC * 16 + chunk_on<KC>(kat, l16, lq, 4 * j);
-          const v8h_t K0 = *reinterpret_cast<const v8h_t *>(k), K1 = *reinterpret_cast<const v8h_t *>(k + 16 * KC * 16);
+          const char *kj = k + chunk_on<KC>(kat, 4 * j);
+          const v8h_t K0 = *reinterpret_cast<const v8h_t *>(kj), K1 = *reinterpret_cast<const v8h_t *>(kj + 1024 * NC);
 #pragma unroll
           for (int i = 0; i < MB; i++) {
             S[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K0, ql[i][j], j ? S[i][0] : zero, 0, 0, 0);
@@ -605,7 +615,7 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
           weights(S[i], c[i], row[i].seen, mask, pos, 4 * t + 2 * half, m[i], l[i], O[i], Ph[i], Pl[i]);
 #pragma unroll
         for (int n = 0; n < ND; n++) {
-          const v8h_t V = v_columns(kb_ + TILE + 32 * half * KC * 16, vat, n);
+          const v8h_t V = v_columns(k + TILE, vat, n);
 #pragma unroll
           for (int i = 0; i < MB; i++) O[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(V, Pl[i], O[i][n], 0, 0, 0);
 #pragma unroll
@@ -621,7 +631,8 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
       for (int n = 0; n < ND; n++)
 #pragma unroll
         for (int e = 0; e < 4; e++) z = fmaf(O[i][n][e], 0.f, z);
-      const bool bad = row[i].there && row[i].seen > job.at(0) && (!(fmaf(l[i], 0.f, z) == 0.f) || m[i] == -INFINITY);
+      const bool none = m[i] == -INFINITY;
+      const bool bad = row[i].there && row[i].seen > job.at(0) && (none || !(fmaf(l[i], 0.f, z) == 0.f));
       const uint64_t all = __ballot(bad);
       const uint32_t slow = (uint32_t)(all | all >> 16 | all >> 32 | all >> 48) & 0xffff;
       if (row[i].there && !(slow >> l16 & 1)) {
@@ -630,7 +641,7 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
 #pragma unroll
         for (int n = 0; n < ND; n++)
           if (16 * n + 4 * lq < a.hd)
-            *reinterpret_cast<v4f_t *>(dst + 16 * n) = m[i] == -INFINITY ? v4f_t{0.f, 0.f, 0.f, 0.f} : O[i][n] * by;
+            *reinterpret_cast<v4f_t *>(dst + 16 * n) = none ? v4f_t{0.f, 0.f, 0.f, 0.f} : O[i][n] * by;
         if (lq == 0) put_ml(row[i], m[i], l[i]);
       }
 #pragma unroll 1
