@@ -105,6 +105,18 @@ __device__ __forceinline__ void wait_dma() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
 }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// The larger of two, one instruction (fmaxf's operands are first made quiet, an
+// instruction each). A NaN may give either: its row shows it in l.
+__device__ __forceinline__ float max2(float x, float y) { return __builtin_amdgcn_fmed3f(x, y, INFINITY); }
+// That over the lanes l, l ^ 16, l ^ 32, l ^ 48, in every one of them.
+__device__ __forceinline__ float row_max(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t x = __builtin_bit_cast(uint32_t, max2(__builtin_bit_cast(float, (uint32_t)a[0]),
+                                                       __builtin_bit_cast(float, (uint32_t)a[1])));
+  const auto c = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return max2(__builtin_bit_cast(float, (uint32_t)c[0]), __builtin_bit_cast(float, (uint32_t)c[1]));
+}
 // Least / most of a row of 16 lanes, in all of them.
 template <bool MOST>
 __device__ __forceinline__ uint32_t row16(uint32_t v) {
@@ -292,13 +304,14 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
   };
   // ---- page ids: lane i holds that of 16-key block id0 + i of the part ----
   uint32_t idv, id0 = 0;
-  bool holes = false;  // a block met so far has no page
+  uint32_t holes = 0;  // (uniform) a block met so far has no page
   auto fetch_ids = [&]() __attribute__((always_inline)) {
     const uint32_t pos = job.at(id0 + lane), i = pos >> a.kv.page_shift;
     idv = i < a.kv.max_pages ? a.kv.page(job.seq, i) : NO_PAGE;
   };
   auto note_holes = [&]() __attribute__((always_inline)) {
-    holes |= __any(idv == NO_PAGE && job.at(id0 + lane) < job.k0 + job.n) != 0;
+    const uint64_t none = __ballot(idv == NO_PAGE && job.at(id0 + lane) < job.k0 + job.n);
+    holes |= __builtin_amdgcn_readfirstlane(none != 0);
   };
   auto block_id = [&](uint32_t i) __attribute__((always_inline)) {  // (uniform)
     if (i - id0 >= 64) {
@@ -323,17 +336,23 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
   auto weights = [&](v4f_t (&S)[2], float c, uint32_t seen, bool mask, uint32_t pos, uint32_t block, float &m, float &l,
                      v4f_t *O, v8h_t &Ph, v8h_t &Pl) __attribute__((always_inline)) {
     if (mask) {  // (uniform)
-      const uint32_t s0 = holes && block_id(block) == NO_PAGE ? 0 : seen;
-      const uint32_t s1 = holes && block_id(block + 1) == NO_PAGE ? 0 : seen;
+      uint32_t s0 = seen, s1 = seen;
+      if (holes) {
+        const auto gone = [&](uint32_t i) {
+          const uint32_t page = job.at(i) >> a.kv.page_shift;
+          return page >= a.kv.max_pages || a.kv.page(job.seq, page) == NO_PAGE;
+        };
+        if (gone(block)) s0 = 0;
+        if (gone(block + 1)) s1 = 0;
+      }
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
 #pragma unroll
         for (int r = 0; r < 4; r++)
           if (pos + 16 * kb + 4 * lq + r >= (kb ? s1 : s0)) S[kb][r] = -INFINITY;
     }
-    float mx = fmaxf(fmaxf(fmaxf(S[0][0], S[0][1]), fmaxf(S[0][2], S[0][3])),
-                     fmaxf(fmaxf(S[1][0], S[1][1]), fmaxf(S[1][2], S[1][3])));
-    mx = quarter_max(mx) * c;
+    const float mx = row_max(max2(max2(max2(S[0][0], S[0][1]), max2(S[0][2], S[0][3])),
+                                  max2(max2(S[1][0], S[1][1]), max2(S[1][2], S[1][3])))) * c;
     if (__any(mx > m + M_LAG)) {  // (also the first visible key: m = -inf)
       const float mn = mx > m + M_LAG ? ceilf(mx) : m;
       const float al = mn == m ? 1.f : m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
@@ -352,7 +371,8 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
         const float p1 = __builtin_amdgcn_exp2f(fmaf(S[kb][r + 1], c, t));
         ps[2 * kb + r / 2] = p0 + p1;
         const v2h_t h = __builtin_convertvector((v2f_t{p0, p1}), v2h_t);
-        const v2h_t w = __builtin_convertvector((v2f_t{p0 - (float)h[0], p1 - (float)h[1]}), v2h_t);
+        const v2h_t w = __builtin_convertvector(
+            (v2f_t{__builtin_fmaf(-1.f, (float)h[0], p0), __builtin_fmaf(-1.f, (float)h[1], p1)}), v2h_t);
         Ph[4 * kb + r] = h[0], Ph[4 * kb + r + 1] = h[1];
         Pl[4 * kb + r] = w[0], Pl[4 * kb + r + 1] = w[1];
       }

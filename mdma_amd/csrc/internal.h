@@ -529,8 +529,9 @@ void *split_space(mdma_ctx *ctx, uint64_t bytes);
 // attn_paged.hip.
 void launch_attn_paged(mdma_ctx *ctx, const float *q, const PagedView &kv, uint32_t n_new, uint32_t q_heads,
                        uint32_t kv_heads, uint32_t hd, float *o);
-// lora.hip. A slot's A is [rank_pad][in_pad], its B [n_out][stride] (stride:
-// its rank in whole 16s), both padded with zeros; rank 0: no adapter.
+// lora.hip. A slot's A is [rank_pad][in_pad] (rank_pad: 16, 32 or whole 64s),
+// its B [n_out][stride] (stride: its rank in whole 16s); values past the rank and the
+// columns are 0 up to stride and in_pad (whole 32s). rank 0: no adapter.
 struct LoraSlot {
   uint32_t rank, stride;
   float scale;

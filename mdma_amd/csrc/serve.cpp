@@ -299,7 +299,9 @@ int mdma_gfx950_lora_new(mdma_ctx *ctx, int32_t dtype, uint64_t n_in, uint64_t n
     auto l = std::make_unique<mdma_lora>();
     l->ctx = ctx;
     l->max_rank = max_rank;
-    const uint64_t eb = type_size(dtype), rp = (max_rank + 15) / 16 * 16, ip = (n_in + 31) / 32 * 32;
+    // (ranks in the blocks that a wave of the shrink kernel takes together)
+    const uint64_t rp = max_rank <= 16 ? 16 : max_rank <= 32 ? 32 : (max_rank + 63) / 64 * 64;
+    const uint64_t eb = type_size(dtype), ip = (n_in + 31) / 32 * 32;
     auto take = [&](uint64_t bytes, mdma_buf **b) {
       const int st = mdma_gfx950_alloc(ctx, bytes, MDMA_POOL_WEIGHTS, b);
       if (st) fail(st, mdma_gfx950_last_error());
@@ -352,7 +354,7 @@ int mdma_gfx950_lora_add(mdma_ctx *ctx, const mdma_lora *l, const mdma_buf *ids,
     std::lock_guard<std::recursive_mutex> g(ctx->lock);
     const LoraView &w = l->view;
     const uint64_t T = new_tokens(op, "x", x, 1, w.n_in);
-    if (T > (1u << 24)) fail(MDMA_ERR_SIZE_OVERFLOW, "lora_add: more than 2^24 tokens");
+    if (T > (1u << 21)) fail(MDMA_ERR_SIZE_OVERFLOW, "lora_add: more than 2^21 tokens");
     const uint64_t out = T * w.n_out * 4;
     check_buf(ctx, op, "x", x, x->len, 16);
     check_buf(ctx, op, "ids", ids, T * 4, 4);
