@@ -442,7 +442,7 @@ int mdma_gfx950_lora_new(mdma_ctx *ctx, int32_t dtype, uint64_t n_in, uint64_t n
 int mdma_gfx950_lora_load(mdma_lora *lora, uint64_t slot, const void *a, const void *b, uint64_t rank, float scale);
 /* y[t] = base[t] + scale * b (a x[t]) with the adapter of slot ids[t] (u32
  * [T]); y[t] = base[t] where ids[t] names no slot, or an empty one. x [T,
- * n_in], base and y [T, n_out] f32, T (at most 2^21) from x's length; y may be base
+ * n_in], base and y [T, n_out] f32, T (at most 2^19) from x's length; y may be base
  * itself. Sums are f32 in an order fixed by the call's sizes and ids. */
 int mdma_gfx950_lora_add(mdma_ctx *ctx, const mdma_lora *lora, const mdma_buf *ids, const mdma_buf *x,
                          const mdma_buf *base, mdma_buf *y);

@@ -530,7 +530,7 @@ void *split_space(mdma_ctx *ctx, uint64_t bytes);
 void launch_attn_paged(mdma_ctx *ctx, const float *q, const PagedView &kv, uint32_t n_new, uint32_t q_heads,
                        uint32_t kv_heads, uint32_t hd, float *o);
 // lora.hip. A slot's A is [rank_pad][in_pad] (rank_pad: 16, 32 or whole 64s),
-// its B [n_out][stride] (stride: its rank in whole 16s); values past the rank and the
+// its B [n_out][stride] (stride: 16, or its rank in whole 32s); values past the rank and the
 // columns are 0 up to stride and in_pad (whole 32s). rank 0: no adapter.
 struct LoraSlot {
   uint32_t rank, stride;
@@ -542,6 +542,7 @@ struct LoraView {
   const void *a, *b;
   const LoraSlot *info;
 };
+constexpr uint64_t LORA_MAX_TOKENS = 1u << 19;  // (16 a row of the grid)
 uint64_t lora_scratch(const LoraView &w, uint64_t T);
 void launch_lora(mdma_ctx *ctx, const LoraView &w, const uint32_t *ids, uint32_t T, const float *x, const float *base,
                  float *y, float *u);

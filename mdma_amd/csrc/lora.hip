@@ -9,10 +9,17 @@
 // its column; at 16 and more tokens a value the f32 rate (64 operations a cycle and
 // SIMD) is still ahead of memory up to rank 64.
 //
-// A wave works for 16 tokens of one adapter (columns of the MFMA). Up to
+// A workgroup works for 16 tokens of one adapter (columns of the MFMA). Up to
 // GATHER tokens they are gathered from the whole batch, so requests in any order read each
-// adapter once per 16 of its tokens; above, a wave takes 16 consecutive tokens and
+// adapter once per 16 of its tokens; above, they are 16 consecutive tokens, and the workgroup
 // goes through the adapters among them one after the other (prompts come in runs).
+//
+// Measured, F16: 32 tokens of 16 adapters of ranks to 64, 4096 -> 14336: 18.7 us (shrink 5.7, expand
+// 12.7; 32 MB, 1.7 TB/s); 2000 tokens in runs, ranks to 32, 4096 -> 4096: 32.2 us (shrink 14.2, expand 18.2;
+// 88 MB, 2.7 TB/s). With a wave for each group of 16 tokens and part, in place of four that share
+// it through LDS, they took 24.6 and 39.0 us.
+#include <type_traits>
+
 #include "kernels.h"
 
 namespace mdma {
@@ -25,7 +32,12 @@ typedef _Float16 v8h_t __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t GATHER = 256;       // a thread a token
 constexpr uint32_t NO_SLOT = ~0u, NO_TOKEN = ~0u;
-constexpr uint32_t COLS = 256;         // outputs of an expand workgroup, 64 a wave and step
+constexpr uint32_t COLS = 256;         // outputs of an expand workgroup at a time, 64 a wave
+
+// Up to 16 tokens of one adapter (NO_TOKEN past the last; none: not a group's lead token).
+struct Group {
+  uint32_t slot, tok[16];
+};
 
 // The slot of token t's adapter, NO_SLOT where it has none.
 __device__ __forceinline__ uint32_t slot_of(const LoraView &w, const uint32_t *ids, uint32_t t) {
@@ -64,273 +76,358 @@ __device__ __forceinline__ bool gather(const LoraView &w, const uint32_t *ids, u
   return true;
 }
 
-// Eight values of a row from column 8 c on, as f32.
+// Eight consecutive values of an adapter's row, from 16 or 32 bytes.
 template <class W>
-struct Eight;
-template <>
-struct Eight<_Float16> {
-  v8h_t v;
-  __device__ __forceinline__ void load(const void *p, uint64_t at) {
-    v = *reinterpret_cast<const v8h_t *>(static_cast<const _Float16 *>(p) + at);
-  }
-  __device__ __forceinline__ float operator[](int i) const { return (float)v[i]; }
-};
-template <>
-struct Eight<float> {
-  v4f_t v[2];
-  __device__ __forceinline__ void load(const void *p, uint64_t at) {
-    const v4f_t *q = reinterpret_cast<const v4f_t *>(static_cast<const float *>(p) + at);
-    v[0] = q[0];
-    v[1] = q[1];
-  }
-  __device__ __forceinline__ float operator[](int i) const { return v[i >> 2][i & 3]; }
-};
-// Four of them.
-__device__ __forceinline__ v4f_t four(const _Float16 *p) {
-  const v4h_t h = *reinterpret_cast<const v4h_t *>(p);
-  return __builtin_convertvector(h, v4f_t);
-}
-__device__ __forceinline__ v4f_t four(const float *p) { return *reinterpret_cast<const v4f_t *>(p); }
-
-// x's eight values from column k on; 0 past the row's end.
-__device__ __forceinline__ void load_x(const float *row, uint32_t k, uint32_t n_in, v4f_t *x) {
-  if (k + 8 <= n_in) {
-    x[0] = *reinterpret_cast<const v4f_u *>(row + k);
-    x[1] = *reinterpret_cast<const v4f_u *>(row + k + 4);
-  } else {
+struct Eight {
+  typedef std::conditional_t<std::is_same_v<W, float>, v4f_t, v8h_t> V;
+  V v[sizeof(W) / 2];
+  __device__ __forceinline__ void load(const W *p) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e >> 2][e & 3] = k + e < n_in ? row[k + e] : 0.f;
+    for (size_t i = 0; i < sizeof(W) / 2; i++) v[i] = reinterpret_cast<const V *>(p)[i];
   }
-}
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (std::is_same_v<W, float>) return v[e >> 2][e & 3];
+    else return (float)v[0][e];
+  }
+};
 
 // The tokens' sums over 32-column steps s0, s0 + by, .. below s1, for ranks
-// r0 + 16 i: D[i] holds ranks 4 lq + (0..3) of token l16.
-template <class W, int RT>
+// r0 + 16 i: D[i] holds ranks 4 lq + (0..3) of token l16. A lane's columns of a step are 8 lq + (0..7).
+// G steps are under way while the last G are multiplied; no branch stands between the loads (where
+// one did, its merge waited for each of them: 2000 tokens x 4096 columns, ranks to 32, 30 us instead of 17).
+template <class W, int RT, int G>
 __device__ __forceinline__ void shrink_steps(const LoraView &w, uint32_t slot, const float *xr, uint32_t r0, uint32_t s0,
                                              uint32_t s1, uint32_t by, v4f_t *D) {
   const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
-  const uint64_t a0 = ((uint64_t)slot * w.rank_pad + r0 + l16) * w.in_pad + 8 * lq;
-  Eight<W> a[RT], an[RT];
-  v4f_t x[2], xn[2];
+  const W *a0 = static_cast<const W *>(w.a) + ((uint64_t)slot * w.rank_pad + r0 + l16) * w.in_pad + 8 * lq;
+  const float *x0 = xr + 8 * lq;
+  Eight<W> a[G][RT], an[G][RT];
+  v4f_t x[G][2], xn[G][2];
 #pragma unroll
   for (int i = 0; i < RT; i++) D[i] = v4f_t{0.f, 0.f, 0.f, 0.f};
-  if (s0 >= s1) return;
-  auto load = [&](uint32_t s, Eight<W> *A, v4f_t *X) __attribute__((always_inline)) {
+  const uint32_t whole = w.n_in / 32, end = min(s1, whole);  // steps without a column past the row's end
+  auto load = [&](uint32_t s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < RT; i++) A[i].load(w.a, a0 + (uint64_t)16 * i * w.in_pad + 32 * s);
-    load_x(xr, 32 * s + 8 * lq, w.n_in, X);
+    for (int g = 0; g < G; g++) {
+      const uint32_t t = min(s + g * by, end - 1);  // (past the end: a step of the part again, with x 0)
+      xn[g][0] = *reinterpret_cast<const v4f_u *>(x0 + 32 * t);
+      xn[g][1] = *reinterpret_cast<const v4f_u *>(x0 + 32 * t + 4);
+#pragma unroll
+      for (int i = 0; i < RT; i++) an[g][i].load(a0 + (uint64_t)16 * i * w.in_pad + 32 * t);
+    }
   };
-  load(s0, an, xn);
-  for (uint32_t s = s0; s < s1; s += by) {
+  auto multiply = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < RT; i++) a[i] = an[i];
-    x[0] = xn[0], x[1] = xn[1];
-    if (s + by < s1) load(s + by, an, xn);
+    for (int g = 0; g < G; g++)
 #pragma unroll
-    for (int e = 0; e < 8; e++)
+      for (int e = 0; e < 8; e++)
 #pragma unroll
-      for (int i = 0; i < RT; i++)
-        D[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][e], x[e >> 2][e & 3], D[i], 0, 0, 0);
+        for (int i = 0; i < RT; i++)
+          D[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[g][i][e], x[g][e >> 2][e & 3], D[i], 0, 0, 0);
+  };
+  if (s0 < end) {
+    load(s0);
+    for (uint32_t s = s0; s < end; s += G * by) {
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const bool in = s + g * by < end;
+#pragma unroll
+        for (int h = 0; h < 2; h++) x[g][h] = in ? xn[g][h] : v4f_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < RT; i++) a[g][i] = an[g][i];
+      }
+      load(min(s + G * by, end - 1));  // (after the last: not used)
+      __builtin_amdgcn_sched_barrier(0);
+      multiply();
+      asm volatile("" ::: "memory");  // (else the loads are moved into the next round, where they are used)
+    }
+  }
+  if (whole >= s0 && whole < s1 && (whole - s0) % by == 0) {  // the last columns, fewer than 32
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        x[g][e >> 2][e & 3] = g == 0 && 32 * whole + 8 * lq + e < w.n_in ? x0[32 * whole + e] : 0.f;
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int i = 0; i < RT; i++) a[g][i].load(a0 + (uint64_t)16 * i * w.in_pad + 32 * whole);
+    multiply();
   }
 }
 
-// GATHERED: workgroup (lead token, part), its waves share the part's columns and add
-// their sums up in LDS. Else workgroup (64 tokens, part), 16 tokens a wave.
+// Workgroup (part of the columns, lead token or 16 tokens): its waves take the part's steps in
+// turn and add their sums up in LDS.
 template <class W, int RT, bool GATHERED>
 __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraView w, const uint32_t *__restrict__ ids, uint32_t T,
                                                           const float *__restrict__ x, float *__restrict__ u,
-                                                          uint32_t part_steps) {
+                                                          uint32_t part_steps, Group *__restrict__ groups) {
   __shared__ uint32_t tok[16];
-  __shared__ v4f_t sums[GATHERED ? 3 : 1][RT][64];
+  __shared__ v4f_t sums[3][RT][64];
   const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t part = blockIdx.x, steps = w.in_pad / 32;
   const uint32_t s0 = part * part_steps, s1 = min(s0 + part_steps, steps);
-  auto store = [&](uint32_t t, uint32_t r0, uint32_t rank, const v4f_t *D) __attribute__((always_inline)) {
-    float *dst = u + ((uint64_t)part * T + t) * w.rank_pad + r0 + 4 * lq;
-#pragma unroll
-    for (int i = 0; i < RT; i++) {
-      v4f_t v = D[i];
-      if (r0 + 16 * i >= rank) break;
-      // (0 past the rank, whatever x holds)
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = r0 + 16 * i + 4 * lq + e < rank ? v[e] : 0.f;
-      *reinterpret_cast<v4f_t *>(dst + 16 * i) = v;
-    }
-  };
-  v4f_t D[RT];
-  if constexpr (GATHERED) {
-    uint32_t slot;
-    if (!gather(w, ids, T, blockIdx.y, tok, &slot) || slot == NO_SLOT) return;
-    const uint32_t rank = w.info[slot].rank, t = tok[l16];
-    const float *xr = x + (uint64_t)(t != NO_TOKEN ? t : tok[0]) * w.n_in;
-    for (uint32_t r0 = 0; r0 < rank; r0 += 16 * RT) {  // (uniform)
-      shrink_steps<W, RT>(w, slot, xr, r0, s0 + wave, s1, 4, D);
+  // (all four waves: barriers; t: the lane's token, NO_TOKEN: not stored, row: one there is)
+  auto one = [&](uint32_t slot, uint32_t t, uint32_t row) __attribute__((always_inline)) {
+    const LoraSlot in = w.info[slot];
+    const float *xr = x + (uint64_t)row * w.n_in;
+    for (uint32_t r0 = 0; r0 < in.rank; r0 += 16 * RT) {  // (uniform)
+      v4f_t D[RT];
+      shrink_steps<W, RT, RT <= 2 ? 2 : 1>(w, slot, xr, r0, s0 + wave, s1, 4, D);
       __syncthreads();
       if (wave) {
 #pragma unroll
         for (int i = 0; i < RT; i++) sums[wave - 1][i][lane] = D[i];
       }
       __syncthreads();
-      if (wave == 0) {
+      if (wave || t == NO_TOKEN) continue;
+      float *dst = u + ((uint64_t)part * T + t) * w.rank_pad + r0 + 4 * lq;
 #pragma unroll
-        for (int i = 0; i < RT; i++) D[i] = (D[i] + sums[0][i][lane]) + (sums[1][i][lane] + sums[2][i][lane]);
-        if (t != NO_TOKEN) store(t, r0, rank, D);
+      for (int i = 0; i < RT; i++) {
+        const uint32_t r = r0 + 16 * i;
+        if (r >= in.stride) break;
+        v4f_t v = (D[i] + sums[0][i][lane]) + (sums[1][i][lane] + sums[2][i][lane]);
+        // (0 past the rank, whatever x holds)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = r + 4 * lq + e < in.rank ? v[e] : 0.f;
+        *reinterpret_cast<v4f_t *>(dst + 16 * i) = v;
       }
     }
+  };
+  if constexpr (GATHERED) {
+    uint32_t slot;
+    const bool lead = gather(w, ids, T, blockIdx.y, tok, &slot);
+    if (part == 0 && threadIdx.x < 16) {  // (for the expand)
+      groups[blockIdx.y].tok[threadIdx.x] = lead ? tok[threadIdx.x] : NO_TOKEN;
+      if (threadIdx.x == 0) groups[blockIdx.y].slot = slot;
+    }
+    if (!lead || slot == NO_SLOT) return;
+    const uint32_t t = tok[l16];
+    one(slot, t, t != NO_TOKEN ? t : tok[0]);
   } else {
-    const uint32_t t = 64 * blockIdx.y + 16 * wave + l16;
-    const uint32_t mine = t < T ? slot_of(w, ids, t) : NO_SLOT;
-    const float *xr = x + (uint64_t)min(t, T - 1) * w.n_in;
+    const uint32_t t = 16 * blockIdx.y + l16, mine = t < T ? slot_of(w, ids, t) : NO_SLOT;
+    uint32_t turn = 0;
     for (uint64_t todo = __ballot(mine != NO_SLOT) & 0xffff; todo;) {
       const uint32_t slot = __builtin_amdgcn_readlane((int)mine, __builtin_ctzll(todo));
       todo &= ~__ballot(mine == slot);
-      const uint32_t rank = w.info[slot].rank;
-      for (uint32_t r0 = 0; r0 < rank; r0 += 16 * RT) {
-        shrink_steps<W, RT>(w, slot, xr, r0, s0, s1, 1, D);
-        if (mine == slot) store(t, r0, rank, D);
-      }
+      if (turn++ % gridDim.z == blockIdx.z) one(slot, mine == slot ? t : NO_TOKEN, min(t, T - 1));
     }
   }
 }
 
-// The outputs n0 + 64 step (64 of them) of a wave's 16 tokens (rows of D; tr: the lane's
-// four, NO_TOKEN for none), u's blocks of 16 ranks as operands U.
-template <class W, int UB>
-__device__ __forceinline__ void expand_cols(const LoraView &w, const W *b0, uint32_t stride, float scale, uint32_t blocks,
-                                            const v4f_t *U, uint32_t n, const uint32_t *tr,
-                                            const float *__restrict__ base, float *__restrict__ y) {
-  // Lane l16 has the four outputs from n on, so it reads their rows of B and writes 16 bytes.
-  v4f_t D[4], old[4];
-  const uint32_t lq = (threadIdx.x & 63) >> 4;
-  const bool whole = n + 4 <= w.n_out;
+// The tokens' u, parts added up in order, into LDS: ranks of token l16 in row l16 of RS floats
+// (0 for no token). All 256 threads; tok: 16 tokens.
+constexpr uint32_t U_PAD = 4;
+template <int UB>
+__device__ __forceinline__ void sum_parts(const LoraView &w, const float *u, uint32_t T, uint32_t parts, uint32_t stride,
+                                          const uint32_t *tok, float *us) {
+  constexpr uint32_t RS = 16 * UB + U_PAD;
+  const uint64_t step = (uint64_t)T * w.rank_pad;
+#pragma unroll 1
+  for (uint32_t r = 4 * (threadIdx.x >> 4); r < stride; r += 64) {
+    const uint32_t i = threadIdx.x & 15, t = tok[i];
+    v4f_t s = {0.f, 0.f, 0.f, 0.f};
+    if (t != NO_TOKEN) {
+      const float *p = u + (uint64_t)t * w.rank_pad + r;
+      for (uint32_t c0 = 0; c0 < parts; c0 += 8) {  // (eight loads at a time; past the last part: it again, not added)
+        v4f_t v[8];
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    old[i] = v4f_t{0.f, 0.f, 0.f, 0.f};
-    if (tr[i] != NO_TOKEN) {
-      const float *p = base + (uint64_t)tr[i] * w.n_out + n;
-      if (whole) old[i] = *reinterpret_cast<const v4f_u *>(p);
-      else
+        for (int c = 0; c < 8; c++) v[c] = *reinterpret_cast<const v4f_t *>(p + min(c0 + c, parts - 1) * step);
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (n + j < w.n_out) old[i][j] = p[j];
+        for (int c = 0; c < 8; c++)
+          if (c0 + c < parts) s += v[c];
+      }
     }
+    *reinterpret_cast<v4f_t *>(us + i * RS + r) = s;
   }
-  v4f_t B[4][UB];
+}
+// A wave's operands from there: ranks 4 lq + (0..3) of token l16 where the adapter has 16 (U[0]),
+// else 32 b + 8 lq + (0..7) in U[2 b], U[2 b + 1].
+template <int UB>
+__device__ __forceinline__ void operands(const float *us, uint32_t stride, v4f_t *U) {
+  constexpr uint32_t RS = 16 * UB + U_PAD;
+  const uint32_t lane = threadIdx.x & 63, lq = lane >> 4;
+  const float *p = us + (lane & 15) * RS + (stride == 16 ? 4 : 8) * lq;
+#pragma unroll
+  for (int b = 0; b < UB; b++) {
+    if (b && (stride == 16 || 16 * (b & ~1) >= (int)stride)) break;
+    U[b] = *reinterpret_cast<const v4f_t *>(p + 16 * (b & ~1) + 4 * (b & 1));
+  }
+}
+
+// D += u B for 32 ranks of four outputs' rows (j: n + j), the lane's eight ranks of each.
+template <class W>
+__device__ __forceinline__ void multiply32(const Eight<W> (&B)[4], const v4f_t *U, v4f_t (&D)[4]) {
+#pragma unroll
+  for (int e = 0; e < 8; e++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) D[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(U[e >> 2][e & 3], B[j][e], D[j], 0, 0, 0);
+}
+
+// A wave's 64 outputs from nb on for 16 tokens (rows of D; tr: the lane's four, NO_TOKEN for
+// none, some: one that is there). Lane l16 has the four outputs n = nb + 4 l16 .., so it reads
+// their rows of B, one after the other in memory, and 16 bytes of base and y. STRIDE: 16, 32,
+// 64, or 0 for any number of 32s.
+template <class W, int UB, int STRIDE>
+__device__ __forceinline__ void expand_cols(const LoraView &w, const LoraSlot &in, const W *b0, const v4f_t *U, uint32_t nb,
+                                            const uint32_t *tr, uint32_t some, const float *base, float *y) {
+  const uint32_t lane = threadIdx.x & 63, lq = lane >> 4, n = nb + 4 * (lane & 15);
+  const uint32_t stride = STRIDE ? STRIDE : in.stride;
+  v4f_t D[4], old[4];
+  const bool whole = nb + 64 <= w.n_out;  // (uniform)
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      old[i] = *reinterpret_cast<const v4f_u *>(base + (uint64_t)(tr[i] != NO_TOKEN ? tr[i] : some) * w.n_out + n);
+  }
+  const W *row[4];
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    const W *row = b0 + (uint64_t)min(n + j, w.n_out - 1) * stride + 4 * lq;
-#pragma unroll
-    for (int b = 0; b < UB; b++)
-      if (b < (int)blocks) B[j][b] = four(row + 16 * b);
+    row[j] = b0 + (uint64_t)min(n + j, w.n_out - 1) * stride;
     D[j] = v4f_t{0.f, 0.f, 0.f, 0.f};
   }
+  if constexpr (STRIDE == 16) {
+    typedef std::conditional_t<std::is_same_v<W, float>, v4f_t, v4h_t> V4;
+    V4 B[4];
 #pragma unroll
-  for (int b = 0; b < UB; b++)
-    if (b < (int)blocks) {  // (uniform)
+    for (int j = 0; j < 4; j++) B[j] = *reinterpret_cast<const V4 *>(row[j] + 4 * lq);
 #pragma unroll
-      for (int e = 0; e < 4; e++)
+    for (int e = 0; e < 4; e++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) D[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(U[b][e], B[j][b][e], D[j], 0, 0, 0);
+      for (int j = 0; j < 4; j++) D[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(U[0][e], (float)B[j][e], D[j], 0, 0, 0);
+  } else if constexpr (STRIDE != 0) {
+    Eight<W> B[STRIDE / 32][4];
+#pragma unroll
+    for (int b = 0; b < STRIDE / 32; b++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) B[b][j].load(row[j] + 32 * b + 8 * lq);
+#pragma unroll
+    for (int b = 0; b < STRIDE / 32; b++) multiply32<W>(B[b], U + 2 * b, D);
+  } else {
+#pragma unroll
+    for (int b = 0; b < UB / 2; b++) {
+      if (32 * b >= (int)stride) break;  // (uniform)
+      Eight<W> B[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) B[j].load(row[j] + 32 * b + 8 * lq);
+      multiply32<W>(B, U + 2 * b, D);
     }
+  }
 #pragma unroll
-  for (int i = 0; i < 4; i++)
-    if (tr[i] != NO_TOKEN) {
+  for (int i = 0; i < 4; i++) {
+    if (tr[i] == NO_TOKEN) continue;
+    float *p = y + (uint64_t)tr[i] * w.n_out + n;
+    if (whole) {
       v4f_t v;
 #pragma unroll
-      for (int j = 0; j < 4; j++) v[j] = fmaf(D[j][i], scale, old[i][j]);
-      float *p = y + (uint64_t)tr[i] * w.n_out + n;
-      if (whole) *reinterpret_cast<v4f_u *>(p) = v;
-      else
+      for (int j = 0; j < 4; j++) v[j] = fmaf(D[j][i], in.scale, old[i][j]);
+      *reinterpret_cast<v4f_u *>(p) = v;
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (n + j < w.n_out) p[j] = v[j];
+      for (int j = 0; j < 4; j++)
+        if (n + j < w.n_out) p[j] = fmaf(D[j][i], in.scale, base[(uint64_t)tr[i] * w.n_out + n + j]);
     }
+  }
+}
+// `steps` times 64 outputs, COLS apart, from nb on.
+template <class W, int UB>
+__device__ __forceinline__ void expand(const LoraView &w, const LoraSlot &in, uint32_t slot, const v4f_t *U, uint32_t nb,
+                                       int steps, const uint32_t *tr, uint32_t some, const float *base, float *y) {
+  const W *b0 = static_cast<const W *>(w.b) + (uint64_t)slot * w.n_out * w.rank_pad;
+  auto all = [&](auto S) __attribute__((always_inline)) {
+    for (int k = 0; k < steps && nb + COLS * k < w.n_out; k++)
+      expand_cols<W, UB, decltype(S)::value>(w, in, b0, U, nb + COLS * k, tr, some, base, y);
+  };
+  if (in.stride == 16) all(std::integral_constant<int, 16>());
+  else if (UB >= 2 && in.stride == 32) all(std::integral_constant<int, UB >= 2 ? 32 : 16>());
+  else if (UB >= 4 && in.stride == 64) all(std::integral_constant<int, UB >= 4 ? 64 : 16>());
+  else if (UB > 4) all(std::integral_constant<int, (UB > 4) ? 0 : 16>());
 }
 // y = base for the lane's tokens, outputs n .. n + 3.
 __device__ __forceinline__ void copy_cols(const LoraView &w, uint32_t n, const uint32_t *tr, const float *base, float *y) {
 #pragma unroll
   for (int i = 0; i < 4; i++)
-    if (tr[i] != NO_TOKEN)
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (n + j < w.n_out) y[(uint64_t)tr[i] * w.n_out + n + j] = base[(uint64_t)tr[i] * w.n_out + n + j];
+    if (tr[i] != NO_TOKEN) {
+      const uint64_t at = (uint64_t)tr[i] * w.n_out + n;
+      if (n + 4 <= w.n_out) *reinterpret_cast<v4f_u *>(y + at) = *reinterpret_cast<const v4f_u *>(base + at);
+      else
+        for (int j = 0; n + j < w.n_out && j < 4; j++) y[at + j] = base[at + j];
+    }
 }
 
-// Workgroup (COLS outputs, tokens): GATHERED, 16 tokens of one adapter, 64 outputs a
-// wave; else 64 tokens, 16 a wave, each all the outputs. UB: blocks of 16 ranks.
+// Workgroup (`steps` times COLS outputs, lead token or 16 tokens). UB: blocks of 16 ranks.
 template <class W, int UB, bool GATHERED>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraView w, const uint32_t *__restrict__ ids, uint32_t T,
-                                                          const float *__restrict__ u, uint32_t parts,
-                                                          const float *__restrict__ base, float *__restrict__ y) {
+                                                          const float *__restrict__ u, uint32_t parts, int steps,
+                                                          const float *base, float *y,
+                                                          const Group *__restrict__ groups) {
+  __shared__ __attribute__((aligned(16))) float us[16 * (16 * UB + U_PAD)];
   __shared__ uint32_t tok[16];
   const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t n0 = COLS * blockIdx.x + 4 * l16;
-  // u of the lane's token (l16), ranks 16 b + 4 lq + (0..3): its parts in order.
-  auto load_u = [&](uint32_t t, uint32_t blocks, v4f_t *U) __attribute__((always_inline)) {
-#pragma unroll
-    for (int b = 0; b < UB; b++) {
-      U[b] = v4f_t{0.f, 0.f, 0.f, 0.f};
-      if (t == NO_TOKEN || b >= (int)blocks) continue;
-      const float *p = u + (uint64_t)t * w.rank_pad + 16 * b + 4 * lq;
-      for (uint32_t c = 0; c < parts; c++) U[b] += *reinterpret_cast<const v4f_t *>(p + (uint64_t)c * T * w.rank_pad);
-    }
-  };
-  v4f_t U[UB];
-  uint32_t tr[4];
-  if constexpr (GATHERED) {
-    uint32_t slot;
-    if (!gather(w, ids, T, blockIdx.y, tok, &slot)) return;
+  const uint32_t nb = COLS * steps * blockIdx.x + 64 * wave;
+  // (all four waves: barriers; tok is written; some: a token that is there)
+  auto one = [&](uint32_t slot, uint32_t some) __attribute__((always_inline)) {
+    uint32_t tr[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) tr[i] = tok[4 * lq + i];
-    const uint32_t n = n0 + 64 * wave;
-    if (n - 4 * l16 >= w.n_out) return;
     if (slot == NO_SLOT) {
-      if (base != y) copy_cols(w, n, tr, base, y);
+      if (base != y)
+        for (int k = 0; k < steps; k++) copy_cols(w, nb + COLS * k + 4 * l16, tr, base, y);
       return;
     }
     const LoraSlot in = w.info[slot];
-    load_u(tok[l16], in.stride / 16, U);
-    expand_cols<W, UB>(w, static_cast<const W *>(w.b) + (uint64_t)slot * w.n_out * w.rank_pad, in.stride, in.scale,
-                       in.stride / 16, U, n, tr, base, y);
+    sum_parts<UB>(w, u, T, parts, in.stride, tok, us);
+    __syncthreads();
+    v4f_t U[UB];
+    operands<UB>(us, in.stride, U);
+    expand<W, UB>(w, in, slot, U, nb, steps, tr, some, base, y);
+  };
+  if constexpr (GATHERED) {
+    const Group &g = groups[blockIdx.y];
+    const uint32_t some = g.tok[0];
+    if (some == NO_TOKEN) return;
+    if (threadIdx.x < 16) tok[threadIdx.x] = g.tok[threadIdx.x];
+    __syncthreads();
+    one(g.slot, some);
   } else {
-    const uint32_t t0 = 64 * blockIdx.y + 16 * wave, t = t0 + l16;
-    const uint32_t mine = t < T ? slot_of(w, ids, t) : NO_SLOT;
-    // (the rows 4 lq + i of this lane: their slots from the lanes that looked them up)
-    uint32_t of[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) of[i] = __shfl((int)mine, 4 * lq + i, 64);
+    const uint32_t t = 16 * blockIdx.y + l16, mine = t < T ? slot_of(w, ids, t) : NO_SLOT;
+    uint32_t turn = 0;
     for (uint64_t todo = __ballot(t < T) & 0xffff; todo;) {
-      const uint32_t slot = __builtin_amdgcn_readlane((int)mine, __builtin_ctzll(todo));
+      const uint32_t first = __builtin_ctzll(todo), slot = __builtin_amdgcn_readlane((int)mine, first);
       todo &= ~__ballot(mine == slot);
-#pragma unroll
-      for (int i = 0; i < 4; i++) tr[i] = of[i] == slot && t0 + 4 * lq + i < T ? t0 + 4 * lq + i : NO_TOKEN;
-      if (slot == NO_SLOT) {
-        if (base != y)
-          for (uint32_t k = 0; k < COLS / 64; k++) copy_cols(w, n0 + 64 * k, tr, base, y);
-        continue;
-      }
-      const LoraSlot in = w.info[slot];
-      load_u(mine == slot ? t : NO_TOKEN, in.stride / 16, U);
-      for (uint32_t k = 0; k < COLS / 64 && n0 - 4 * l16 + 64 * k < w.n_out; k++)
-        expand_cols<W, UB>(w, static_cast<const W *>(w.b) + (uint64_t)slot * w.n_out * w.rank_pad, in.stride, in.scale,
-                           in.stride / 16, U, n0 + 64 * k, tr, base, y);
+      if (turn++ % gridDim.z != blockIdx.z) continue;
+      __syncthreads();  // (the last adapter's reads of tok and us)
+      if (threadIdx.x < 16) tok[l16] = mine == slot && t < T ? t : NO_TOKEN;
+      __syncthreads();
+      one(slot, 16 * blockIdx.y + first);
     }
   }
 }
 
 struct Plan {
-  uint32_t steps, parts;  // 32-column steps of a part of n_in, and parts
+  uint32_t groups, turns;  // workgroups of tokens: by lead token, or 16 tokens each
+  uint32_t part_steps, parts;  // 32-column steps of a part of n_in, and parts
+  int steps;                   // times COLS outputs of an expand workgroup
 };
-// Gathered: a part of 256 columns, two steps a wave, at most 16 parts (the
-// expand adds them up). Consecutive: as many parts as keep about 4 waves a SIMD busy, at most 8.
 Plan plan_of(const LoraView &w, uint64_t T) {
-  const uint32_t steps = w.in_pad / 32;
-  const uint64_t most = T <= GATHER ? 16 : std::min<uint64_t>(8, std::max<uint64_t>(1, 4096 * 16 / T));
-  const uint32_t parts = (uint32_t)std::min<uint64_t>(most, (steps + 7) / 8);
-  const uint32_t per = (steps + parts - 1) / parts;
-  return Plan{per, (steps + per - 1) / per};
+  Plan p;
+  const bool gathered = T <= GATHER;
+  p.groups = (uint32_t)(gathered ? T : (T + 15) / 16);
+  // Two workgroups in turn for the adapters among 16 tokens: where one request's tokens end
+  // and another's begin, one that did both was the last by far.
+  p.turns = gathered ? 1 : 2;
+  // Parts of 256 columns, two steps a wave, at most 16 (the expand adds them up); with many
+  // tokens as few as keep 2048 workgroups.
+  const uint32_t all = w.in_pad / 32;
+  const uint64_t most = gathered ? 16 : std::min<uint64_t>(8, std::max<uint64_t>(1, 2048 / p.groups));
+  const uint32_t parts = (uint32_t)std::min<uint64_t>(most, (all + 7) / 8);
+  p.part_steps = (all + parts - 1) / parts;
+  p.parts = (all + p.part_steps - 1) / p.part_steps;
+  const uint64_t cols = (w.n_out + COLS - 1) / COLS;
+  p.steps = (int)std::min<uint64_t>(8, std::max<uint64_t>(1, cols * p.groups / 2048));
+  return p;
 }
 
 template <class W, int UB>
@@ -338,14 +435,15 @@ void launch(mdma_ctx *ctx, const LoraView &w, const uint32_t *ids, uint32_t T, c
             float *y, float *u) {
   constexpr int RT = UB < 4 ? UB : 4;
   const Plan p = plan_of(w, T);
-  const uint32_t cols = (w.n_out + COLS - 1) / COLS;
+  Group *g = reinterpret_cast<Group *>(u + (uint64_t)T * w.rank_pad * p.parts);
+  const uint32_t cols = COLS * p.steps, blocks = (w.n_out + cols - 1) / cols;
+  const dim3 shrink(p.parts, p.groups, p.turns), expand(blocks, p.groups, p.turns);
   if (T <= GATHER) {
-    lora_shrink_kernel<W, RT, true><<<dim3(p.parts, T), 256, 0, ctx->stream>>>(w, ids, T, x, u, p.steps);
-    lora_expand_kernel<W, UB, true><<<dim3(cols, T), 256, 0, ctx->stream>>>(w, ids, T, u, p.parts, base, y);
+    lora_shrink_kernel<W, RT, true><<<shrink, 256, 0, ctx->stream>>>(w, ids, T, x, u, p.part_steps, g);
+    lora_expand_kernel<W, UB, true><<<expand, 256, 0, ctx->stream>>>(w, ids, T, u, p.parts, p.steps, base, y, g);
   } else {
-    const uint32_t tiles = (T + 63) / 64;
-    lora_shrink_kernel<W, RT, false><<<dim3(p.parts, tiles), 256, 0, ctx->stream>>>(w, ids, T, x, u, p.steps);
-    lora_expand_kernel<W, UB, false><<<dim3(cols, tiles), 256, 0, ctx->stream>>>(w, ids, T, u, p.parts, base, y);
+    lora_shrink_kernel<W, RT, false><<<shrink, 256, 0, ctx->stream>>>(w, ids, T, x, u, p.part_steps, g);
+    lora_expand_kernel<W, UB, false><<<expand, 256, 0, ctx->stream>>>(w, ids, T, u, p.parts, p.steps, base, y, g);
   }
 }
 template <class W>
@@ -359,7 +457,7 @@ void launch_of(mdma_ctx *ctx, const LoraView &w, const uint32_t *ids, uint32_t T
 
 }  // namespace
 
-uint64_t lora_scratch(const LoraView &w, uint64_t T) { return T * w.rank_pad * 4 * plan_of(w, T).parts; }
+uint64_t lora_scratch(const LoraView &w, uint64_t T) { return T * w.rank_pad * 4 * plan_of(w, T).parts + GATHER * sizeof(Group); }
 
 void launch_lora(mdma_ctx *ctx, const LoraView &w, const uint32_t *ids, uint32_t T, const float *x, const float *base,
                  float *y, float *u) {

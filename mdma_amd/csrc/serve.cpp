@@ -326,8 +326,8 @@ int mdma_gfx950_lora_load(mdma_lora *l, uint64_t slot, const void *a, const void
     if (rank > l->max_rank) shape_fail("lora_load: rank above max_rank");
     std::lock_guard<std::recursive_mutex> g(l->ctx->lock);
     OnDevice dev(l->ctx);
-    const uint64_t eb = type_size(w.dtype), stride = (rank + 15) / 16 * 16;
-    // Rows padded with zeros: columns to in_pad, ranks to whole 16s.
+    const uint64_t eb = type_size(w.dtype), stride = rank <= 16 ? (rank + 15) / 16 * 16 : (rank + 31) / 32 * 32;
+    // Rows padded with zeros: columns to in_pad, ranks to 16 or whole 32s.
     std::vector<char> pa(stride * w.in_pad * eb), pb(w.n_out * stride * eb);
     for (uint64_t r = 0; r < rank; r++)
       memcpy(&pa[r * w.in_pad * eb], static_cast<const char *>(a) + r * w.n_in * eb, w.n_in * eb);
@@ -354,7 +354,7 @@ int mdma_gfx950_lora_add(mdma_ctx *ctx, const mdma_lora *l, const mdma_buf *ids,
     std::lock_guard<std::recursive_mutex> g(ctx->lock);
     const LoraView &w = l->view;
     const uint64_t T = new_tokens(op, "x", x, 1, w.n_in);
-    if (T > (1u << 21)) fail(MDMA_ERR_SIZE_OVERFLOW, "lora_add: more than 2^21 tokens");
+    if (T > LORA_MAX_TOKENS) fail(MDMA_ERR_SIZE_OVERFLOW, "lora_add: more than 2^19 tokens");
     const uint64_t out = T * w.n_out * 4;
     check_buf(ctx, op, "x", x, x->len, 16);
     check_buf(ctx, op, "ids", ids, T * 4, 4);
