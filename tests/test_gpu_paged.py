@@ -143,6 +143,42 @@ def test_largest_batch_of_sequences(backend):
     c.check()
 
 
+@pytest.mark.parametrize("S,P,M", [(64, 8192, 128), (64, 8193, 64), (65, 8191, 127), (3, 24583, 2731), (1024, 8200, 8)])
+def test_books_of_many_pages(backend, S, P, M):
+    """Tables and counts about and past what one workgroup holds (8192 entries, 8192 pages); scattered live pages."""
+    r = np.random.default_rng(S)
+    c = Cache(backend, ref.Books(P, 16, S, M), 1, 8, S)
+    b = c.books
+    ids, at = r.permutation(P), 0
+    for s in range(S):
+        b.lens[s] = r.integers(0, min(M, P // S - 1) * 16 - 20)
+        u = b.used(b.lens[s])
+        b.table[s, :u] = ids[at:at + u]
+        b.refs[ids[at:at + u]] += 1
+        at += u
+    for dev, host in ((c.dev.table, b.table), (c.dev.lens, b.lens), (c.dev.refs, b.refs)):
+        backend.upload(dev, 0, host)
+    status, live = backend.alloc(4 * S), backend.alloc(4)
+    for step in range(2):
+        f = np.where(r.random(S) < 0.6, np.arange(S), r.integers(0, S, S)).astype(np.uint32)
+        backend.kv_pages_fork(c.dev, buf(backend, f))
+        b.fork(f)
+        c.check((step, "fork"))
+        g = r.integers(0, 20, S).astype(np.uint32)
+        backend.kv_pages_grow(c.dev, buf(backend, g), status)
+        want, copies = b.grow(g)
+        assert np.array_equal(u32(backend, status, S), want)
+        for pool in (c.k, c.v):
+            ref.apply(pool, copies=copies)
+        c.check((step, "grow"))
+        backend.kv_pages_compact(c.dev, live)
+        L, moves = b.compact()
+        for pool in (c.k, c.v):
+            ref.apply(pool, moves=moves)
+        assert u32(backend, live, 1)[0] == L
+        c.check((step, "compact"))
+
+
 def test_ids_outside_the_pool_are_skipped(backend):
     b, _ = filled([40, 33], 16, 5)
     b.table[0, 1] = b.P  # one past the last page
