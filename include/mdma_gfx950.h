@@ -415,8 +415,9 @@ int mdma_gfx950_kv_pages_compact(mdma_ctx *ctx, const mdma_kv_pages *pages, mdma
  * sequence s is position lens[s] - n_new + j (its room made by kv_pages_grow
  * before), q rotated in place, the rotated k and v stored in layer's pages
  * (rounded to f16; k itself is not changed). The angles are rope's: the f32
- * product of the position and the f32 frequency. A token before position 0
- * (an empty slot of a padded batch) is left alone. */
+ * product of the position and the f32 frequency, from a table as long as max_pages
+ * reaches (at most 2^24 positions). A token before position 0 (an empty slot of a
+ * padded batch) is left alone. */
 int mdma_gfx950_rope_kv_write_paged(mdma_ctx *ctx, mdma_buf *q, const mdma_buf *k, const mdma_buf *v,
                                     const mdma_kv_pages *pages, uint64_t layer, const mdma_rope_spec *spec);
 /* Causal attention of the batch's last n_new tokens (n_new from q's length):

@@ -36,6 +36,7 @@ typedef short v4s_t __attribute__((ext_vector_type(4)));
 
 constexpr float P_BITS = 10.f, M_LAG = 5.f;
 constexpr uint32_t MAX_PARTS = 64;  // parts of a row: a lane each in the joining kernel
+constexpr uint64_t PART_BYTES = 256ull << 20;  // of all parts: with more rows than they fit, fewer parts
 constexpr uint32_t BLOCK = 128;     // keys: part c of P takes the blocks c, c + P, c + 2 P, .. of its job
 
 // n / d for n < 2^31, by a multiplication.
@@ -745,16 +746,17 @@ void launch_attn_paged(mdma_ctx *ctx, const float *q, const PagedView &kv, uint3
   // A prefix of a few tiles is read again by each sequence instead.
   const bool shared = kv.n_seqs > 1 && pre >= 256;
   uint64_t parts_bytes = 0;
+  const uint64_t most_slots = PART_BYTES / ((uint64_t)a.rows * (hd + 2) * 4);
   auto plan = [&](bool split) {
-    a.start = split && shared ? (uint32_t)pre : 0;
+    a.start = split && shared && most_slots >= 2 ? (uint32_t)pre : 0;
     const uint64_t units = (uint64_t)kv.n_seqs * kv_heads * rt_t, keys = cap - a.start;
     a.n_p = a.n_t = 1;
     if (a.start)
-      a.n_p = (uint32_t)std::min<uint64_t>({MAX_PARTS / 2, tiles(pre, 2 * BLOCK),
+      a.n_p = (uint32_t)std::min<uint64_t>({MAX_PARTS / 2, most_slots / 2, tiles(pre, 2 * BLOCK),
                                             std::max<uint64_t>(1, want / 2 / ((uint64_t)kv_heads * rt_p))});
     else a.n_p = 0;
-    if (split && keys > 768)
-      a.n_t = (uint32_t)std::min<uint64_t>({MAX_PARTS / 2, tiles(keys, 2 * BLOCK),
+    if (split && keys > 768 && most_slots > a.n_p + 1)
+      a.n_t = (uint32_t)std::min<uint64_t>({MAX_PARTS / 2, most_slots - a.n_p, tiles(keys, 2 * BLOCK),
                                             std::max<uint64_t>(tiles(keys, 512), tiles(want * 3 / 2, units))});
     const uint32_t slots = a.n_p + a.n_t;
     parts_bytes = slots > 1 ? (uint64_t)slots * a.rows * (hd + 2) * 4 : 0;

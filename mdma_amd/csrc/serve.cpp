@@ -237,6 +237,9 @@ int mdma_gfx950_rope_kv_write_paged(mdma_ctx *ctx, mdma_buf *q, const mdma_buf *
     check_buf(ctx, op, "q", q, q->len, 16);
     const uint64_t q_heads = q->len / (rows * hd * 4);
     if (rows > INT32_MAX || q_heads * hd > (1u << 24)) fail(MDMA_ERR_SIZE_OVERFLOW, "rope_kv_write_paged: too many rows");
+    // (a position is a factor in f32; the table of angles reaches to the end of the page table)
+    if ((uint64_t)b.max_pages << b.page_shift > 1u << 24)
+      fail(MDMA_ERR_SIZE_OVERFLOW, "rope_kv_write_paged: max_pages reaches past 2^24 positions");
     check_books_apart(op, pages, {q, k, v});
     check_apart(op, "q", q, q->len, k);
     check_apart(op, "q", q, q->len, v);

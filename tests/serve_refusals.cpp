@@ -120,6 +120,11 @@ int main() {
   write("empty q", SHAPE, &empty, &nk, &nv, 0, &rope);
   write("q is k", SHAPE, &nk, &nk, &nv, 0, &rope);
   write("q in the pool", SHAPE, &k, &nk, &nv, 0, &rope);
+  mdma_buf long_table = mk(3ull * ((1 << 20) + 1) * 4);
+  P far = good;
+  far.table = &long_table;
+  far.max_pages = (1 << 20) + 1;  // 16 positions past 2^24
+  expect("positions past 2^24", OVER, mdma_gfx950_rope_kv_write_paged(&ctx, &q, &nk, &nv, &far, 0, &rope));
   // attn
   auto attn = [&](const char *what, int code, const mdma_buf *aq, uint64_t layer, const mdma_buf *pre, mdma_attn_spec s,
                   mdma_buf *ao) { expect(what, code, mdma_gfx950_attn_paged(&ctx, aq, &good, layer, pre, &s, ao)); };

@@ -420,6 +420,30 @@ def test_attn_paged_pages_that_are_not_there(backend):
     assert not got[1].any()
 
 
+@pytest.mark.parametrize("S,new,lens", [(1, 1025, [1900]), (2, 1025, [1900, 1100]), (1, 2100, [2200])])
+def test_attn_paged_more_rows_than_parts_have_room_for(backend, S, new, lens):
+    """Rows whose parts would take hundreds of MB: fewer parts, in the end none, and the prefix read by each sequence.
+    Some rows of each wave against 64 bits."""
+    heads, hd, page, prefix_pages = 64, 256, 64, 8
+    b, pre = filled(lens, page, 5, prefix_pages=prefix_pages)
+    c = Cache(backend, b, 1, hd, 6)
+    r = np.random.default_rng(7)
+    q = r.standard_normal((S, new, heads * hd), np.float32)
+    ob = backend.alloc(q.nbytes)
+    backend.attn_paged(buf(backend, q), c.dev, 0, buf(backend, pre), AttnSpec(hd, heads, 1), ob)
+    o = backend.download_f32(ob).reshape(S, new, heads, hd)
+    assert np.isfinite(o).all()
+    q = q.reshape(o.shape)
+    for s in range(S):
+        for j in [0, 1, 2, 15, 16, new // 2, new - 2, new - 1]:
+            # (one query of a shorter sequence: the same keys)
+            one, at = ref.Books(b.P, page, 1, b.M), int(b.lens[s]) - new + j + 1
+            one.table[0], one.lens[0] = b.table[s], at
+            h = r.integers(0, heads, 3)
+            want, tol = ref.attn(q[s, j, h].reshape(1, 1, -1), c.k, c.v, one, 0, 3, 1)
+            assert np.all(np.abs(o[s, j, h].reshape(1, 1, -1) - want) <= tol), (s, j, h)
+
+
 def test_attn_paged_no_prefix_equals_prefix(backend):
     """The same cache with its shared pages named and not: within the bound of either."""
     b, pre = filled([300, 280, 1, 500], 16, 8, prefix_pages=10)
