@@ -15,8 +15,8 @@
 // goes through the adapters among them one after the other (prompts come in runs).
 //
 // Measured, F16: 32 tokens of 16 adapters of ranks to 64, 4096 -> 14336: 18.7 us (shrink 5.7, expand
-// 12.7; 32 MB, 1.7 TB/s); 2000 tokens in runs, ranks to 32, 4096 -> 4096: 32.2 us (shrink 14.2, expand 18.2;
-// 88 MB, 2.7 TB/s). With a wave for each group of 16 tokens and part, in place of four that share
+// 12.7; 32 MB, 1.7 TB/s); 2000 tokens in runs, ranks to 32, 4096 -> 4096: 31.7 us (shrink 13.1, expand 18.1;
+// 88 MB, 2.8 TB/s); 20000 tokens 213 us (1 GB, 4.6 TB/s, a large copy's rate). With a wave for each group of 16 tokens and part, in place of four that share
 // it through LDS, they took 24.6 and 39.0 us.
 #include <type_traits>
 
@@ -418,10 +418,12 @@ Plan plan_of(const LoraView &w, uint64_t T) {
   // Two workgroups in turn for the adapters among 16 tokens: where one request's tokens end
   // and another's begin, one that did both was the last by far.
   p.turns = gathered ? 1 : 2;
-  // Parts of 256 columns, two steps a wave, at most 16 (the expand adds them up); with many
-  // tokens as few as keep 2048 workgroups.
+  // Parts of 256 columns, two steps a wave, at most 16 (the expand adds them up: 32 tokens x 4096
+  // columns 18.0 us, with 4 parts 21.1); with many tokens at most 8, and as few as make 512
+  // workgroups, but two (x 4096 columns: 2000 tokens 30.6 us with 4, 31.5 with 8, 36.5 with 2; 8000
+  // tokens 98 us with 2, 102 with 1).
   const uint32_t all = w.in_pad / 32;
-  const uint64_t most = gathered ? 16 : std::min<uint64_t>(8, std::max<uint64_t>(1, 2048 / p.groups));
+  const uint64_t most = gathered ? 16 : std::min<uint64_t>(8, std::max<uint64_t>(2, 512 / p.groups));
   const uint32_t parts = (uint32_t)std::min<uint64_t>(most, (all + 7) / 8);
   p.part_steps = (all + parts - 1) / parts;
   p.parts = (all + p.part_steps - 1) / p.part_steps;
