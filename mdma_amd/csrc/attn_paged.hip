@@ -268,7 +268,7 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void attn_paged_kernel(Args a
     x.head = job.kvh * a.by_group.d + c - t * a.by_group.d;
     if (job.is_p) {
       const uint32_t s = a.by_new(x.token);
-      x.seen = seen_by(a.kv.length(s), a.n_new, x.token - s * a.n_new);
+      x.seen = min(seen_by(a.kv.length(s), a.n_new, x.token - s * a.n_new), a.start);  // (the rest: the tail's)
     } else {
       x.seen = seen_by(job.len, a.n_new, t);
     }

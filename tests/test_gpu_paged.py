@@ -332,6 +332,18 @@ def test_attn_paged_long(backend, lens, new, page, heads, kv_heads, hd, prefix_p
     check_attn(backend, lens, new, page, heads, kv_heads, hd, prefix_pages, seed=5)
 
 
+@pytest.mark.parametrize("page,prefix_pages", [(16, 17), (16, 21), (16, 30), (32, 9), (32, 13), (64, 5), (128, 3)])
+@pytest.mark.parametrize("S,new,heads,kv_heads,hd", [(2, 1, 4, 2, 64), (5, 3, 8, 2, 96), (9, 2, 16, 2, 128),
+                                                     (3, 40, 4, 2, 128), (6, 3, 8, 1, 256)])
+def test_attn_paged_prefix_that_ends_inside_a_tile(backend, page, prefix_pages, S, new, heads, kv_heads, hd):
+    """A shared prefix of any number of pages, few query rows and many: no key behind it counts twice. Tails of one
+    position to a few pages, and sequences that end in the prefix."""
+    pre = page * prefix_pages
+    lens = [pre + new + i * 17 % 70 for i in range(S)]
+    lens[-1] = pre - 5 if S > 2 else pre + new
+    check_attn(backend, lens, new, page, heads, kv_heads, hd, prefix_pages)
+
+
 def test_attn_paged_wide_scores(backend):
     """Queries forty times larger: a few keys take all the weight."""
     check_attn(backend, [700, 33, 290], 2, 16, 8, 2, 64, 1, qscale=40.0)
