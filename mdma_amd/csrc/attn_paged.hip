@@ -19,6 +19,11 @@
 //    p, and 2^-35 of the row's largest p.
 // m is a whole number, so 2^(m - m') is a power of two: rescaling l and O
 // and joining chunks round nothing.
+//
+// Measured, 32 heads of 128 over 8 KV heads: 64 sequences of one token behind 16384 shared keys and up
+// to 1000 of their own 66 us (186 MB; a wave's 64-key tile for 32 rows takes 2.3 us, products and
+// softmax one after the other); 16 of 4096 keys, nothing shared, 47 us (5.7 TB/s); 16 of 5 tokens
+// over up to 4096 keys 18 us, 4 of them the join; a prompt of 1000 tokens behind 3000 keys 192 us.
 #include <type_traits>
 
 #include "kernels.h"
@@ -743,8 +748,11 @@ void launch_attn_paged(mdma_ctx *ctx, const float *q, const PagedView &kv, uint3
   a.by_rt_t = Div(rt_t);
   a.by_rt_p = Div(rt_p);
   const uint64_t want = 2ull * ctx->cu_count;  // workgroups that fill the chip
-  // A prefix of a few tiles is read again by each sequence instead.
-  const bool shared = kv.n_seqs > 1 && pre >= 256;
+  // A short prefix is read again by each sequence instead (mostly from the caches). One token each, 32
+  // heads of 128 over 8, shared against not: 32 sequences behind 512 keys 21 and 10 us, behind 1024
+  // 22 and 18, behind 2048 23 and 30, behind 8192 30 and 85; 64 behind 1024 25 and 31; 8 behind 1024
+  // 11.7 and 11.1, behind 2048 12 and 16.
+  const bool shared = kv.n_seqs > 1 && pre >= 1024;
   uint64_t parts_bytes = 0;
   const uint64_t most_slots = PART_BYTES / ((uint64_t)a.rows * (hd + 2) * 4);
   auto plan = [&](bool split) {
@@ -755,9 +763,16 @@ void launch_attn_paged(mdma_ctx *ctx, const float *q, const PagedView &kv, uint3
       a.n_p = (uint32_t)std::min<uint64_t>({MAX_PARTS / 2, most_slots / 2, tiles(pre, 2 * BLOCK),
                                             std::max<uint64_t>(1, want / 2 / ((uint64_t)kv_heads * rt_p))});
     else a.n_p = 0;
-    if (split && keys > 768 && most_slots > a.n_p + 1)
+    // (keys: what the table has room for, the lengths are the device's. One token each: 1 or 8 sequences of
+    // 512 keys take 9.3 us split, 8.3 whole, of 1000 keys 9.5 and 12; where the sequences fill the chip by
+    // themselves, 64 with up to 1000 keys 23 and 19, up to 4096 42 and 53, not beside a prefix's
+    // workgroups: 66 and 71. Keys a part, at most, for lengths of every size: 16 sequences of 5 tokens over up to
+    // 4096 keys 18 us with 512, 23 with 1024; 64 of one token 44 and 42, 64 of 4096 keys each 207 and 199.)
+    const bool full = !a.start && units >= want;
+    if (split && keys > (full ? 2048u : 768u) && most_slots > a.n_p + 1)
       a.n_t = (uint32_t)std::min<uint64_t>({MAX_PARTS / 2, most_slots - a.n_p, tiles(keys, 2 * BLOCK),
-                                            std::max<uint64_t>(tiles(keys, 512), tiles(want * 3 / 2, units))});
+                                            std::max<uint64_t>(tiles(keys, full ? 1024 : 512),
+                                                               tiles(want * 3 / 2, units))});
     const uint32_t slots = a.n_p + a.n_t;
     parts_bytes = slots > 1 ? (uint64_t)slots * a.rows * (hd + 2) * 4 : 0;
   };

@@ -109,6 +109,24 @@ def test_many_tokens(backend, dtype, tokens, pattern):
     check(backend, dtype, 320, 200, 32, [8 + i % 25 for i in range(slots)], ids, seed=tokens)
 
 
+def test_most_tokens_of_a_call(backend):
+    """2^19 tokens; one more is refused."""
+    T, r = 1 << 19, np.random.default_rng(3)
+    st = Set(backend, GGML_F16, 8, 8, 4, [4, 2, 0], 5)
+    ids = r.choice([0, 1, 2, NONE], T).astype(np.uint32)
+    x, base = (r.standard_normal((T, 8), np.float32) for _ in range(2))
+    got = run(backend, st, ids, x, base)
+    at = np.concatenate([np.arange(40), r.integers(0, T, 200), np.arange(T - 40, T)])
+    want, tol = st.want(ids[at], x[at], base[at])
+    assert np.all(np.abs(got[at] - want) <= tol)
+    bare = ids >= 2
+    assert np.array_equal(got[bare].view(np.uint32), base[bare].view(np.uint32))
+    n = T + 1
+    with pytest.raises(BackendError) as e:
+        backend.lora_add(st.dev, backend.alloc(4 * n), backend.alloc(32 * n), backend.alloc(32 * n), backend.alloc(32 * n))
+    assert "2^19" in str(e.value)
+
+
 def test_token_alone_and_in_a_batch(backend):
     """A token's result in a batch of 40 against the same token alone: both within the bound, and the same call twice
     the same bits."""

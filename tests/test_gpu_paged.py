@@ -344,6 +344,83 @@ def test_attn_paged_prefix_that_ends_inside_a_tile(backend, page, prefix_pages, 
     check_attn(backend, lens, new, page, heads, kv_heads, hd, prefix_pages)
 
 
+# (prefixes long enough to be read once for the batch)
+LONG_PREFIX = [(16, 64), (16, 65), (16, 67), (16, 70), (32, 33), (64, 17), (128, 9), (256, 5)]
+
+
+@pytest.mark.parametrize("page,prefix_pages", LONG_PREFIX)
+@pytest.mark.parametrize("S,new,heads,kv_heads,hd", [(2, 1, 4, 2, 64), (3, 3, 8, 2, 96), (9, 2, 16, 2, 128),
+                                                     (3, 40, 2, 1, 128), (6, 3, 8, 1, 256), (5, 2, 6, 6, 48)])
+def test_attn_paged_long_prefix(backend, page, prefix_pages, S, new, heads, kv_heads, hd):
+    pre = page * prefix_pages
+    lens = [pre + new + i * 17 % 70 for i in range(S)]
+    lens[-1] = pre - 5 if S > 2 else pre + new
+    if S > 3:
+        lens[1], lens[2] = 0, 500
+    check_attn(backend, lens, new, page, heads, kv_heads, hd, prefix_pages)
+
+
+@pytest.mark.parametrize("page,prefix_pages", LONG_PREFIX)
+@pytest.mark.parametrize("S,new,heads,kv_heads", [(3, 1, 8, 2), (24, 3, 8, 2)])
+def test_attn_paged_long_prefix_beside_anything(backend, page, prefix_pages, S, new, heads, kv_heads):
+    """NaN in pages of no one, behind every sequence's end and in the other layer, infinities where a prefix list
+    names no page: none of it is read into a row."""
+    pre = page * prefix_pages
+    lens = [pre + new + i * 5 % 37 for i in range(S)]
+    lens[1] = pre - page - 3
+
+    def mutate(b, c, q):
+        held = np.zeros((b.P, b.pl), bool)
+        for s in range(b.S):
+            p, row, _ = ref.positions(b, s)
+            held[p, row] = True
+        for pool in (c.k, c.v):
+            pool[:, ~held] = np.nan
+            pool[0] = np.inf
+    check_attn(backend, lens, new, page, heads, kv_heads, 64, prefix_pages, mutate=mutate)
+    # Pages of the prefix that are not there: page 0, of no one, holds NaN.
+    b, ids = filled(lens, page, 3, prefix_pages=prefix_pages)
+    c = Cache(backend, b, 1, kv_heads * 64, 4)
+    ids = ids.copy()
+    gone = [0, 3, prefix_pages - 1]
+    c.k[0, ids[gone]], c.v[0, ids[gone]] = np.nan, -np.inf
+    c = Cache(backend, b, 1, kv_heads * 64, 4, c.k, c.v)
+    ids[gone] = [b.P, ref.NONE, 0x80000000]
+    q = np.random.default_rng(5).standard_normal((S, new, heads * 64)).astype(np.float32)
+    want, tol = ref.attn(q, c.k, c.v, b, 0, heads, kv_heads, ids)
+    assert np.all(np.abs(run_attn(backend, c, q, heads, kv_heads, 0, ids) - want) <= tol)
+
+
+@pytest.mark.parametrize("S", [2, 40])
+def test_attn_paged_long_prefix_values_that_are_not_finite(backend, S):
+    """An infinite value in the shared prefix makes its dim infinite for every row that sees it, a NaN key the row NaN;
+    a sequence that ends before them has neither."""
+    page, pages = 32, 40
+    for k_bad in (False, True):
+        lens = [page * pages + 1 + i % 7 for i in range(S - 1)] + [1100]
+        b, ids = filled(lens, page, 3, prefix_pages=pages)
+        c = Cache(backend, b, 1, 64, 4)
+        if k_bad:
+            c.k[0, ids[37], 9, 3] = np.nan
+        else:
+            c.v[0, ids[37], 9, 7] = np.inf
+        c = Cache(backend, b, 1, 64, 4, c.k, c.v)
+        q = np.random.default_rng(6).standard_normal((S, 1, 128)).astype(np.float32)
+        got = run_attn(backend, c, q, 2, 1, 0, ids)
+        (c.k if k_bad else c.v)[0, ids[37], 9] = np.where(np.isfinite((c.k if k_bad else c.v)[0, ids[37], 9]),
+                                                          (c.k if k_bad else c.v)[0, ids[37], 9], 0)
+        want, tol = ref.attn(q, c.k, c.v, b, 0, 2, 1, ids)
+        assert np.all(np.abs(got - want)[-1] <= tol[-1])
+        if k_bad:
+            assert np.all(np.isnan(got[:-1]))
+        else:
+            got = got.reshape(S, 2, 64)
+            assert np.all(got[:-1, :, 7] == np.inf)
+            assert np.all(np.isfinite(np.delete(got[:-1], 7, -1)))
+            other = np.abs(got - want.reshape(got.shape))[:-1] <= tol.reshape(got.shape)[:-1]
+            assert np.all(np.delete(other, 7, -1))
+
+
 def test_attn_paged_wide_scores(backend):
     """Queries forty times larger: a few keys take all the weight."""
     check_attn(backend, [700, 33, 290], 2, 16, 8, 2, 64, 1, qscale=40.0)
