@@ -34,7 +34,7 @@ constexpr uint32_t GATHER = 256;       // a thread a token
 constexpr uint32_t NO_SLOT = ~0u, NO_TOKEN = ~0u;
 constexpr uint32_t COLS = 256;         // outputs of an expand workgroup at a time, 64 a wave
 
-// Up to 16 tokens of one adapter (NO_TOKEN past the last; none: not a group's lead token).
+// Up to 16 tokens of one adapter (NO_TOKEN past the last; none at all: no such group).
 struct Group {
   uint32_t slot, tok[16];
 };
@@ -45,33 +45,50 @@ __device__ __forceinline__ uint32_t slot_of(const LoraView &w, const uint32_t *i
   return id < w.n_slots && w.info[id].rank ? id : NO_SLOT;
 }
 
-// Up to GATHER tokens: the tokens of the adapter of token `lead`, from its rank among
-// them on (a multiple of 16, else false: another workgroup's), 16 at most, into tok.
-__device__ __forceinline__ bool gather(const LoraView &w, const uint32_t *ids, uint32_t T, uint32_t lead,
+// Up to GATHER tokens, in groups: 16 at most of one adapter, in their order; a group's number is that of
+// its first token among the groups' first ones. Group `index` into tok, its adapter into *slot; false past
+// the last. (Numbered without gaps: the workgroups of one launch with something to do are consecutive, and
+// so on different CUs. By the number of the first token itself, 85 tokens of one adapter, whose groups start
+// every 16, met on the same few: rank 8, 14336 -> 4096, the call took 28.6 us, so 11.9; 32 tokens of 16
+// adapters, whose first tokens are consecutive anyway, 18.1 and 18.4.)
+__device__ __forceinline__ bool gather(const LoraView &w, const uint32_t *ids, uint32_t T, uint32_t index,
                                        uint32_t *tok, uint32_t *slot) {
-  __shared__ uint32_t all[GATHER];
+  __shared__ __attribute__((aligned(16))) uint32_t all[GATHER];
   __shared__ uint64_t mask[GATHER / 64];
-  const uint32_t t = threadIdx.x, wave = t >> 6;
+  __shared__ uint32_t found[2];
+  const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t mine = t < T ? slot_of(w, ids, t) : NO_SLOT;
   all[t] = mine;
   if (t < 16) tok[t] = NO_TOKEN;
   __syncthreads();
-  *slot = __builtin_amdgcn_readfirstlane(all[lead]);
-  const bool same = t < T && mine == *slot;
-  const uint64_t m = __ballot(same);
+  uint32_t rank = 0;  // among the tokens of its adapter
+  for (uint32_t i = 0; i < 64 * wave + 64 && i < T; i += 32) {  // (eight reads at a time)
+    uint4 l[8];
+#pragma unroll
+    for (int c = 0; c < 8; c++) l[c] = *reinterpret_cast<const uint4 *>(all + i + 4 * c);
+    uint32_t same = 0;
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+      same |= ((l[c].x == mine) | (l[c].y == mine) << 1 | (l[c].z == mine) << 2 | (uint32_t)(l[c].w == mine) << 3) << 4 * c;
+    if (t > i) rank += __popc(t - i < 32 ? same & ((1u << (t - i)) - 1) : same);
+  }
+  const bool lead = t < T && rank % 16 == 0;
+  const uint64_t m = __ballot(lead);
   if ((t & 63) == 0) mask[wave] = m;
   __syncthreads();
-  uint32_t before = 0, lead_rank = 0;
+  uint32_t before = __popcll(m & ((1ull << (t & 63)) - 1)), groups = 0;
 #pragma unroll
   for (uint32_t v = 0; v < GATHER / 64; v++) {
-    const uint64_t x = mask[v];
-    if (v < wave) before += __popcll(x);
-    if (v < lead / 64) lead_rank += __popcll(x);
-    else if (v == lead / 64) lead_rank += __popcll(x & ((1ull << (lead & 63)) - 1));
+    const uint32_t n = __popcll(mask[v]);
+    if (v < wave) before += n;
+    groups += n;
   }
-  if (lead_rank % 16) return false;
-  const uint32_t rank = before + __popcll(m & ((1ull << (t & 63)) - 1));
-  if (same && rank >= lead_rank && rank < lead_rank + 16) tok[rank - lead_rank] = t;
+  if (index >= groups) return false;  // (uniform)
+  if (lead && before == index) found[0] = mine, found[1] = rank;
+  __syncthreads();
+  *slot = __builtin_amdgcn_readfirstlane(found[0]);
+  const uint32_t first = __builtin_amdgcn_readfirstlane(found[1]);
+  if (t < T && mine == *slot && rank >= first && rank < first + 16) tok[rank - first] = t;
   __syncthreads();
   return true;
 }
@@ -156,7 +173,7 @@ __device__ __forceinline__ void shrink_steps(const LoraView &w, uint32_t slot, c
   }
 }
 
-// Workgroup (part of the columns, lead token or 16 tokens): its waves take the part's steps in
+// Workgroup (part of the columns, group or 16 tokens): its waves take the part's steps in
 // turn and add their sums up in LDS.
 template <class W, int RT, bool GATHERED>
 __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraView w, const uint32_t *__restrict__ ids, uint32_t T,
@@ -197,12 +214,12 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraView w, const uint
   };
   if constexpr (GATHERED) {
     uint32_t slot;
-    const bool lead = gather(w, ids, T, blockIdx.y, tok, &slot);
+    const bool some = gather(w, ids, T, blockIdx.y, tok, &slot);
     if (part == 0 && threadIdx.x < 16) {  // (for the expand)
-      groups[blockIdx.y].tok[threadIdx.x] = lead ? tok[threadIdx.x] : NO_TOKEN;
-      if (threadIdx.x == 0) groups[blockIdx.y].slot = slot;
+      groups[blockIdx.y].tok[threadIdx.x] = some ? tok[threadIdx.x] : NO_TOKEN;
+      if (threadIdx.x == 0 && some) groups[blockIdx.y].slot = slot;
     }
-    if (!lead || slot == NO_SLOT) return;
+    if (!some || slot == NO_SLOT) return;
     const uint32_t t = tok[l16];
     one(slot, t, t != NO_TOKEN ? t : tok[0]);
   } else {
@@ -356,7 +373,7 @@ __device__ __forceinline__ void copy_cols(const LoraView &w, uint32_t n, const u
     }
 }
 
-// Workgroup (`steps` times COLS outputs, lead token or 16 tokens). UB: blocks of 16 ranks.
+// Workgroup (`steps` times COLS outputs, group or 16 tokens). UB: blocks of 16 ranks.
 template <class W, int UB, bool GATHERED>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraView w, const uint32_t *__restrict__ ids, uint32_t T,
                                                           const float *__restrict__ u, uint32_t parts, int steps,
@@ -407,14 +424,15 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraView w, const uint
 }
 
 struct Plan {
-  uint32_t groups, turns;  // workgroups of tokens: by lead token, or 16 tokens each
+  uint32_t groups, turns;  // groups of tokens (at most, up to GATHER tokens), workgroups for each
   uint32_t part_steps, parts;  // 32-column steps of a part of n_in, and parts
   int steps;                   // times COLS outputs of an expand workgroup
 };
 Plan plan_of(const LoraView &w, uint64_t T) {
   Plan p;
   const bool gathered = T <= GATHER;
-  p.groups = (uint32_t)(gathered ? T : (T + 15) / 16);
+  // (every adapter, and none, may end with a group that is not full)
+  p.groups = (uint32_t)(gathered ? std::min<uint64_t>(T, w.n_slots + 1 + T / 16) : (T + 15) / 16);
   // Two workgroups in turn for the adapters among 16 tokens: where one request's tokens end
   // and another's begin, one that did both was the last by far.
   p.turns = gathered ? 1 : 2;

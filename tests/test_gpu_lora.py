@@ -109,6 +109,15 @@ def test_many_tokens(backend, dtype, tokens, pattern):
     check(backend, dtype, 320, 200, 32, [8 + i % 25 for i in range(slots)], ids, seed=tokens)
 
 
+@pytest.mark.parametrize("counts", [(17, 17, 1), (1, 1, 1), (16, 16, 16), (33, 1, 17), (81, 81, 81), (1, 0, 255),
+                                    (49, 129, 65), (0, 256, 0)])
+def test_groups_of_an_adapter_that_are_not_full(backend, counts):
+    """Tokens of two adapters and of none, as many of each as these, in runs and mixed."""
+    ids = np.repeat(np.array([0, 1, NONE], np.uint32), counts)
+    check(backend, GGML_F16, 96, 130, 8, [8, 5], ids, seed=3)
+    check(backend, GGML_F16, 96, 130, 8, [8, 5], np.random.default_rng(4).permutation(ids), seed=3)
+
+
 def test_most_tokens_of_a_call(backend):
     """2^19 tokens; one more is refused."""
     T, r = 1 << 19, np.random.default_rng(3)
