@@ -5,7 +5,10 @@
 //
 // The tables are a few KB to a few MB, so the calls are bound by launches and
 // by the latency of one workgroup's scans; the copies they cause (a shared
-// last page, a page moved) run on the whole chip, in 16-byte pieces.
+// last page, a page moved) run on the whole chip, in 16-byte pieces. Measured: fork and grow of 8
+// sequences 12 us in three launches (2.2, 3.9, 1.6); of 64 with 56 last pages of 8 layers to copy
+// (37 MB) 17 us (3.2, 5.9, 8.5); compact of 2048 pages, 259 MB to move, 4.7 and 43 us (6 TB/s, part of
+// it in the cache); the rotated write of 2000 tokens, 92 MB, 15.6 us.
 #include "kernels.h"
 #include "paged.h"
 
@@ -40,7 +43,7 @@ __device__ __forceinline__ uint32_t scan_wg(uint32_t v, uint32_t *total) {
 
 // Which of the ids p .. p + 7 have holders, a bit each: a thread's share of BOOK_WG * 8 ids that
 // are counted with one scan. (With a scan for each BOOK_WG ids and kind the plan of compact took
-// 5.0 us at 200 pages, so 4.2.)
+// 5.0 us at 200 pages, so 3.6 to 4.2.)
 __device__ __forceinline__ uint32_t held_bits(const uint32_t *refs, uint32_t n_pages, uint32_t p) {
   typedef uint32_t v4u_u __attribute__((ext_vector_type(4), aligned(4)));
   uint32_t bits = 0;

@@ -14,8 +14,8 @@
 // adapter once per 16 of its tokens; above, they are 16 consecutive tokens, and the workgroup
 // goes through the adapters among them one after the other (prompts come in runs).
 //
-// Measured, F16: 32 tokens of 16 adapters of ranks to 64, 4096 -> 14336: 18.7 us (shrink 5.7, expand
-// 12.7; 32 MB, 1.7 TB/s); 2000 tokens in runs, ranks to 32, 4096 -> 4096: 31.7 us (shrink 13.1, expand 18.1;
+// Measured, F16: 32 tokens of 16 adapters of ranks to 64, 4096 -> 14336: 19.1 us (shrink 7.6, expand
+// 11.2; 32 MB, 1.7 TB/s); 2000 tokens in runs, ranks to 32, 4096 -> 4096: 31.7 us (shrink 13.1, expand 18.1;
 // 88 MB, 2.8 TB/s); 20000 tokens 213 us (1 GB, 4.6 TB/s, a large copy's rate). With a wave for each group of 16 tokens and part, in place of four that share
 // it through LDS, they took 24.6 and 39.0 us.
 #include <type_traits>
