@@ -118,6 +118,21 @@ def test_groups_of_an_adapter_that_are_not_full(backend, counts):
     check(backend, GGML_F16, 96, 130, 8, [8, 5], np.random.default_rng(4).permutation(ids), seed=3)
 
 
+@pytest.mark.parametrize("seed", range(30))
+def test_any_sizes(backend, seed):
+    """Sizes, ranks and who has which adapter drawn at random."""
+    r = np.random.default_rng(2000 + seed)
+    n_in, n_out = (int(np.exp(r.uniform(0, np.log(3000)))) for _ in range(2))
+    tokens = int(np.exp(r.uniform(0, np.log(700))))
+    top = int(r.choice([1, 7, 16, 17, 32, 33, 64, 65, 130, 256]))
+    ranks = [int(k) for k in r.integers(0, top + 1, int(r.integers(1, 9)))]
+    ids = r.choice(list(range(len(ranks) + 1)) + [NONE], tokens)
+    if r.random() < 0.5:
+        ids = np.sort(ids)
+    check(backend, GGML_F16 if r.random() < 0.6 else GGML_F32, n_in, n_out, top, ranks, ids, seed=seed,
+          in_place=bool(r.random() < 0.5))
+
+
 def test_most_tokens_of_a_call(backend):
     """2^19 tokens; one more is refused."""
     T, r = 1 << 19, np.random.default_rng(3)

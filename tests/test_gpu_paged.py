@@ -421,6 +421,23 @@ def test_attn_paged_long_prefix_values_that_are_not_finite(backend, S):
             assert np.all(np.delete(other, 7, -1))
 
 
+@pytest.mark.parametrize("seed", range(40))
+def test_attn_paged_any_sizes(backend, seed):
+    """Sizes, lengths (around the prefix's end, below new, 0) and prefixes drawn at random."""
+    r = np.random.default_rng(1000 + seed)
+    heads, kv_heads, hd = [(2, 1, 8), (6, 6, 48), (8, 2, 64), (7, 1, 128), (4, 1, 256), (6, 2, 80), (12, 2, 24),
+                           (34, 2, 72)][r.integers(8)]
+    page, new = int(2 ** r.integers(4, 9)), int(r.choice([1, 1, 2, 3, 9, 33]))
+    S = int(r.integers(1, 1 + (12 if new < 4 else 4)))
+    prefix_pages = int(r.choice([0, r.integers(1, 300 // page + 2), r.integers(1024 // page, 1500 // page + 2)]))
+    pre = prefix_pages * page
+    lens = [int(pre + r.choice([0, 1, new, r.integers(1, 40), r.integers(1, 700)])) for _ in range(S)]
+    for s in range(S):
+        if r.random() < 0.2:
+            lens[s] = int(r.choice([0, 1, max(0, new - 1), max(0, pre - 1), r.integers(0, pre + 1)]))
+    check_attn(backend, lens, new, page, heads, kv_heads, hd, prefix_pages, seed=seed)
+
+
 def test_attn_paged_wide_scores(backend):
     """Queries forty times larger: a few keys take all the weight."""
     check_attn(backend, [700, 33, 290], 2, 16, 8, 2, 64, 1, qscale=40.0)
