@@ -9,10 +9,12 @@
 // its column; at 16 and more tokens a value the f32 rate (64 operations a cycle and
 // SIMD) is still ahead of memory up to rank 64.
 //
-// A workgroup works for 16 tokens of one adapter (columns of the MFMA). Up to
-// GATHER tokens they are gathered from the whole batch, so requests in any order read each
-// adapter once per 16 of its tokens; above, they are 16 consecutive tokens, and the workgroup
-// goes through the adapters among them one after the other (prompts come in runs).
+// A workgroup works for 16 tokens of one adapter (columns of the MFMA). Up to GROUP_MOST tokens they are
+// gathered from the whole batch, so requests in any order read each adapter once per 16 of its
+// tokens: by every workgroup itself up to GATHER, else by a launch before. Above, they are 16 consecutive
+// tokens, and the workgroup goes through the adapters among them one after the other (prompts come in
+// runs). 4096 -> 4096, rank 16, 16 adapters, gathered against consecutive: 64 tokens in runs 9.2 and 13.5 us,
+// mixed 9.2 and 41; 512 in runs 14.2 and 10.9, mixed 13.8 and 66; 1000 22.9 and 22.7, mixed 22 and 131.
 //
 // Measured, F16: 32 tokens of 16 adapters of ranks to 64, 4096 -> 14336: 19.1 us (shrink 7.6, expand
 // 11.2; 32 MB, 1.7 TB/s); 2000 tokens in runs, ranks to 32, 4096 -> 4096: 31.7 us (shrink 13.1, expand 18.1;
@@ -31,6 +33,9 @@ typedef _Float16 v4h_t __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h_t __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t GATHER = 256;       // a thread a token
+constexpr uint32_t GROUP_MOST = 1024;  // tokens that lora_groups_kernel takes, a thread a token
+// Who finds a workgroup's tokens: it itself, lora_groups_kernel before it, or they are 16 consecutive ones.
+enum How { GATHERED, GIVEN, CONSECUTIVE };
 constexpr uint32_t NO_SLOT = ~0u, NO_TOKEN = ~0u;
 constexpr uint32_t COLS = 256;         // outputs of an expand workgroup at a time, 64 a wave
 
@@ -91,6 +96,51 @@ __device__ __forceinline__ bool gather(const LoraView &w, const uint32_t *ids, u
   if (t < T && mine == *slot && rank >= first && rank < first + 16) tok[rank - first] = t;
   __syncthreads();
   return true;
+}
+
+// The groups of up to GROUP_MOST tokens, one workgroup: the adapters met in a hash table, a token's place
+// among its adapter's from a counter there (in any order: a token's sums do not depend on its group).
+// most: groups there is room for, all of which are written.
+__global__ __launch_bounds__(GROUP_MOST) void lora_groups_kernel(LoraView w, const uint32_t *__restrict__ ids, uint32_t T,
+                                                                 Group *__restrict__ groups, uint32_t most) {
+  constexpr uint32_t SIZE = 2 * GROUP_MOST, EMPTY = ~0u - 1;
+  __shared__ uint32_t key[SIZE], count[SIZE], wsum[GROUP_MOST / 64];
+  const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  for (uint32_t i = t; i < SIZE; i += GROUP_MOST) key[i] = EMPTY, count[i] = 0;
+  for (uint32_t i = t; i < 16 * most; i += GROUP_MOST) groups[i / 16].tok[i % 16] = NO_TOKEN;
+  __syncthreads();
+  uint32_t mine = NO_SLOT, at = 0, rank = 0;
+  if (t < T) {
+    mine = slot_of(w, ids, t);
+    // (at most T keys in twice as many places: one is found)
+    for (at = mine * 0x9e3779b1u >> 21;; at = (at + 1) % SIZE) {
+      const uint32_t was = atomicCAS(key + at, EMPTY, mine);
+      if (was == EMPTY || was == mine) break;
+    }
+    rank = atomicAdd(count + at, 1u);
+  }
+  __syncthreads();
+  // The groups before each entry's: a scan, two entries a thread.
+  const uint32_t n0 = (count[2 * t] + 15) / 16, n1 = (count[2 * t + 1] + 15) / 16;
+  uint32_t x = n0 + n1;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t y = __shfl_up(x, d, 64);
+    if (lane >= (uint32_t)d) x += y;
+  }
+  if (lane == 63) wsum[wave] = x;
+  __threadfence_block();
+  __syncthreads();  // (counts are read, the groups' tokens cleared)
+  uint32_t before = x - n0 - n1;
+  for (uint32_t v = 0; v < wave; v++) before += wsum[v];
+  count[2 * t] = before;
+  count[2 * t + 1] = before + n0;
+  __syncthreads();
+  if (t < T) {
+    const uint32_t g = count[at] + rank / 16;  // (below most: an entry's last group alone is not full)
+    groups[g].tok[rank % 16] = t;
+    groups[g].slot = mine;
+  }
 }
 
 // Eight consecutive values of an adapter's row, from 16 or 32 bytes.
@@ -175,7 +225,7 @@ __device__ __forceinline__ void shrink_steps(const LoraView &w, uint32_t slot, c
 
 // Workgroup (part of the columns, group or 16 tokens): its waves take the part's steps in
 // turn and add their sums up in LDS.
-template <class W, int RT, bool GATHERED>
+template <class W, int RT, How HOW>
 __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraView w, const uint32_t *__restrict__ ids, uint32_t T,
                                                           const float *__restrict__ x, float *__restrict__ u,
                                                           uint32_t part_steps, Group *__restrict__ groups) {
@@ -212,7 +262,13 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraView w, const uint
       }
     }
   };
-  if constexpr (GATHERED) {
+  if constexpr (HOW == GIVEN) {
+    const Group &g = groups[blockIdx.y];
+    const uint32_t some = g.tok[0];
+    if (some == NO_TOKEN || g.slot == NO_SLOT) return;
+    const uint32_t t = g.tok[l16];
+    one(g.slot, t, t != NO_TOKEN ? t : some);
+  } else if constexpr (HOW == GATHERED) {
     uint32_t slot;
     const bool some = gather(w, ids, T, blockIdx.y, tok, &slot);
     if (part == 0 && threadIdx.x < 16) {  // (for the expand)
@@ -374,7 +430,7 @@ __device__ __forceinline__ void copy_cols(const LoraView &w, uint32_t n, const u
 }
 
 // Workgroup (`steps` times COLS outputs, group or 16 tokens). UB: blocks of 16 ranks.
-template <class W, int UB, bool GATHERED>
+template <class W, int UB, How HOW>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraView w, const uint32_t *__restrict__ ids, uint32_t T,
                                                           const float *__restrict__ u, uint32_t parts, int steps,
                                                           const float *base, float *y,
@@ -401,7 +457,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraView w, const uint
     operands<UB>(us, in.stride, U);
     expand<W, UB>(w, in, slot, U, nb, steps, tr, some, base, y);
   };
-  if constexpr (GATHERED) {
+  if constexpr (HOW != CONSECUTIVE) {
     const Group &g = groups[blockIdx.y];
     const uint32_t some = g.tok[0];
     if (some == NO_TOKEN) return;
@@ -424,24 +480,24 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraView w, const uint
 }
 
 struct Plan {
-  uint32_t groups, turns;  // groups of tokens (at most, up to GATHER tokens), workgroups for each
+  uint32_t groups, turns;  // groups of tokens (at most, up to GROUP_MOST tokens), workgroups for each
   uint32_t part_steps, parts;  // 32-column steps of a part of n_in, and parts
   int steps;                   // times COLS outputs of an expand workgroup
 };
 Plan plan_of(const LoraView &w, uint64_t T) {
   Plan p;
-  const bool gathered = T <= GATHER;
+  const bool grouped = T <= GROUP_MOST;
   // (every adapter, and none, may end with a group that is not full)
-  p.groups = (uint32_t)(gathered ? std::min<uint64_t>(T, w.n_slots + 1 + T / 16) : (T + 15) / 16);
+  p.groups = (uint32_t)(grouped ? std::min<uint64_t>(T, w.n_slots + 1 + T / 16) : (T + 15) / 16);
   // Two workgroups in turn for the adapters among 16 tokens: where one request's tokens end
   // and another's begin, one that did both was the last by far.
-  p.turns = gathered ? 1 : 2;
+  p.turns = grouped ? 1 : 2;
   // Parts of 256 columns, two steps a wave, at most 16 (the expand adds them up: 32 tokens x 4096
   // columns 18.0 us, with 4 parts 21.1); with many tokens at most 8, and as few as make 512
   // workgroups, but two (x 4096 columns: 2000 tokens 30.6 us with 4, 31.5 with 8, 36.5 with 2; 8000
   // tokens 98 us with 2, 102 with 1).
   const uint32_t all = w.in_pad / 32;
-  const uint64_t most = gathered ? 16 : std::min<uint64_t>(8, std::max<uint64_t>(2, 512 / p.groups));
+  const uint64_t most = T <= GATHER ? 16 : std::min<uint64_t>(8, std::max<uint64_t>(2, 512 / p.groups));
   const uint32_t parts = (uint32_t)std::min<uint64_t>(most, (all + 7) / 8);
   p.part_steps = (all + parts - 1) / parts;
   p.parts = (all + p.part_steps - 1) / p.part_steps;
@@ -458,13 +514,15 @@ void launch(mdma_ctx *ctx, const LoraView &w, const uint32_t *ids, uint32_t T, c
   Group *g = reinterpret_cast<Group *>(u + (uint64_t)T * w.rank_pad * p.parts);
   const uint32_t cols = COLS * p.steps, blocks = (w.n_out + cols - 1) / cols;
   const dim3 shrink(p.parts, p.groups, p.turns), expand(blocks, p.groups, p.turns);
-  if (T <= GATHER) {
-    lora_shrink_kernel<W, RT, true><<<shrink, 256, 0, ctx->stream>>>(w, ids, T, x, u, p.part_steps, g);
-    lora_expand_kernel<W, UB, true><<<expand, 256, 0, ctx->stream>>>(w, ids, T, u, p.parts, p.steps, base, y, g);
-  } else {
-    lora_shrink_kernel<W, RT, false><<<shrink, 256, 0, ctx->stream>>>(w, ids, T, x, u, p.part_steps, g);
-    lora_expand_kernel<W, UB, false><<<expand, 256, 0, ctx->stream>>>(w, ids, T, u, p.parts, p.steps, base, y, g);
-  }
+  auto run = [&](auto how) {
+    constexpr How HOW = (How)decltype(how)::value;
+    if (HOW == GIVEN) lora_groups_kernel<<<1, GROUP_MOST, 0, ctx->stream>>>(w, ids, T, g, p.groups);
+    lora_shrink_kernel<W, RT, HOW><<<shrink, 256, 0, ctx->stream>>>(w, ids, T, x, u, p.part_steps, g);
+    lora_expand_kernel<W, UB, HOW><<<expand, 256, 0, ctx->stream>>>(w, ids, T, u, p.parts, p.steps, base, y, g);
+  };
+  if (T <= GATHER) run(std::integral_constant<int, GATHERED>());
+  else if (T <= GROUP_MOST) run(std::integral_constant<int, GIVEN>());
+  else run(std::integral_constant<int, CONSECUTIVE>());
 }
 template <class W>
 void launch_of(mdma_ctx *ctx, const LoraView &w, const uint32_t *ids, uint32_t T, const float *x, const float *base,
@@ -477,7 +535,7 @@ void launch_of(mdma_ctx *ctx, const LoraView &w, const uint32_t *ids, uint32_t T
 
 }  // namespace
 
-uint64_t lora_scratch(const LoraView &w, uint64_t T) { return T * w.rank_pad * 4 * plan_of(w, T).parts + GATHER * sizeof(Group); }
+uint64_t lora_scratch(const LoraView &w, uint64_t T) { return T * w.rank_pad * 4 * plan_of(w, T).parts + GROUP_MOST * sizeof(Group); }
 
 void launch_lora(mdma_ctx *ctx, const LoraView &w, const uint32_t *ids, uint32_t T, const float *x, const float *base,
                  float *y, float *u) {

@@ -133,6 +133,19 @@ def test_any_sizes(backend, seed):
           in_place=bool(r.random() < 0.5))
 
 
+@pytest.mark.parametrize("tokens", [256, 257, 300, 1000, 1023, 1024, 1025])
+@pytest.mark.parametrize("slots", [1, 3, 40, 700])
+def test_mixed_requests_same_call_same_bits(backend, tokens, slots):
+    """Every token another request's, around the sizes at which groups are found another way."""
+    r = np.random.default_rng(tokens + slots)
+    ranks = [int(k) for k in r.integers(0, 9, slots)]
+    ids = r.choice(list(range(slots)) + [NONE], tokens)
+    st, got = check(backend, GGML_F16, 64, 70, 8, ranks, ids, seed=slots)
+    x, base = r.standard_normal((tokens, 64), np.float32), r.standard_normal((tokens, 70), np.float32)
+    a, b = (run(backend, st, ids, x, base) for _ in range(2))
+    assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
+
+
 def test_most_tokens_of_a_call(backend):
     """2^19 tokens; one more is refused."""
     T, r = 1 << 19, np.random.default_rng(3)
